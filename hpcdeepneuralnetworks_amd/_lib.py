@@ -19,6 +19,9 @@ OP_FT_SGEMM = 2
 OP_FT_SGEMM_CM_NT = 5
 OP_SGEMV = 3
 OP_OFFLINE_FT_SGEMM = 4
+OP_LAYER_NORM_GRAD = 6
+OP_EXPERT_SORT = 7
+F32, F16, BF16 = 0, 1, 2
 OFFLINE_FT_PANEL_K = 256
 FT_TILE_M = 256
 FT_TILE_N = 128
@@ -55,6 +58,14 @@ EXPORTS = (
     "hpcdnn_offline_ft_sgemm_scalar",
     "hpcdnn_saxpy",
     "hpcdnn_sdot",
+    "hpcdnn_layer_norm",
+    "hpcdnn_layer_norm_grad",
+    "hpcdnn_w4_gemv",
+    "hpcdnn_w4_quantize",
+    "hpcdnn_expert_sort",
+    "hpcdnn_expert_gather",
+    "hpcdnn_expert_combine",
+    "hpcdnn_expert_combine_grad",
     "hpcdnn_workspace_bytes",
     "hpcdnn_workspace_init",
     "hpcdnn_fill_uniform",
@@ -166,6 +177,22 @@ def lib():
     L.hpcdnn_saxpy.argtypes = [i64, f, fp, fp, vp]
     L.hpcdnn_sdot.restype = i
     L.hpcdnn_sdot.argtypes = [i64, fp, fp, fp, vp, sz, vp]
+    L.hpcdnn_layer_norm.restype = i
+    L.hpcdnn_layer_norm.argtypes = [i, i, i, i, vp, i64, vp, vp, f, vp, i64, vp, vp, vp]
+    L.hpcdnn_layer_norm_grad.restype = i
+    L.hpcdnn_layer_norm_grad.argtypes = [i, i, i, i, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, sz, vp]
+    L.hpcdnn_w4_gemv.restype = i
+    L.hpcdnn_w4_gemv.argtypes = [i, i, i, i, i, f, vp, i64, vp, vp, i64, vp, i64, f, vp, i64, vp]
+    L.hpcdnn_w4_quantize.restype = i
+    L.hpcdnn_w4_quantize.argtypes = [i, i, i, i, vp, i64, vp, i64, vp, vp, i64]
+    L.hpcdnn_expert_sort.restype = i
+    L.hpcdnn_expert_sort.argtypes = [i, i, i, vp, i64, vp, vp, vp, vp, sz, vp]
+    L.hpcdnn_expert_gather.restype = i
+    L.hpcdnn_expert_gather.argtypes = [i, i, i, i, i, vp, i64, vp, vp, i64, vp]
+    L.hpcdnn_expert_combine.restype = i
+    L.hpcdnn_expert_combine.argtypes = [i, i, i, i, i, vp, i64, vp, vp, vp, i64, vp]
+    L.hpcdnn_expert_combine_grad.restype = i
+    L.hpcdnn_expert_combine_grad.argtypes = [i, i, i, i, i, vp, i64, vp, i64, vp, vp, vp, i64, vp, vp]
     L.hpcdnn_workspace_bytes.restype = sz
     L.hpcdnn_workspace_bytes.argtypes = [i, i, i, i]
     L.hpcdnn_workspace_init.restype = i

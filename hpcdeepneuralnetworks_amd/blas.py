@@ -358,6 +358,193 @@ def sdot(n: int, x: torch.Tensor, y: torch.Tensor, out: torch.Tensor, ws: torch.
     check(_lib.lib().hpcdnn_sdot(n, px, py, po, ws.data_ptr(), ws.numel() * 4, _stream()), "hpcdnn_sdot")
 
 
+# ---- layer operators ---------------------------------------------------------
+# Tensors of one call are float32, float16 or bfloat16 throughout (parameters of the norms and router weights may or
+# must be float32), on the current device; rows may be strided, columns are contiguous.
+
+_TYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+LAYER_NORM_MAX_COLS = 16384
+W4_GROUPS = (32, 64, 128)
+EXPERTS_MAX = 512
+EXPERTS_MAX_TOPK = 64
+
+
+def _type(t: torch.Tensor, name: str) -> int:
+    if not isinstance(t, torch.Tensor) or t.dtype not in _TYPES:
+        raise HpcdnnError(f"{name} must be a float32, float16 or bfloat16 tensor")
+    return _TYPES[t.dtype]
+
+
+def _on_device(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype):
+        raise HpcdnnError(f"{name} must be a {dtype} tensor on the GPU")
+    if t.device.index != torch.cuda.current_device():
+        raise HpcdnnError(f"{name} is on {t.device}, which is not the current device")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, rows: int, cols: int, name: str, dtype: torch.dtype):
+    """Pointer and row stride of a 2-D tensor with contiguous columns."""
+    ptr = _on_device(t, name, dtype)
+    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < cols:
+        raise HpcdnnError(f"{name} must be 2-D with at least {rows}x{cols} elements, got {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise HpcdnnError(f"{name} must have contiguous columns")
+    return ptr, t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _flat(t: torch.Tensor | None, n: int, name: str, dtype: torch.dtype):
+    """Pointer of a contiguous tensor of at least n elements, None for None."""
+    if t is None:
+        return None
+    ptr = _on_device(t, name, dtype)
+    if t.numel() < n or not t.is_contiguous():
+        raise HpcdnnError(f"{name} must be contiguous with at least {n} elements")
+    return ptr
+
+
+def _scratch(ws: torch.Tensor | None):
+    if ws is None:
+        return None, 0
+    if not (ws.is_cuda and ws.is_contiguous()) or ws.device.index != torch.cuda.current_device():
+        raise HpcdnnError("ws must be a contiguous tensor on the current device")
+    return ws.data_ptr(), ws.numel() * ws.element_size()
+
+
+def _param_type(params, dtype: torch.dtype) -> torch.dtype:
+    kinds = {p.dtype for p in params if p is not None}
+    if not kinds:
+        return torch.float32
+    if len(kinds) > 1 or not kinds <= {torch.float32, dtype}:
+        raise HpcdnnError("w, b and their gradients must share one type: float32 or that of the rows")
+    return kinds.pop()
+
+
+def layer_norm(rows: int, cols: int, x: torch.Tensor, w: torch.Tensor | None, b: torch.Tensor | None, eps: float,
+               y: torch.Tensor, mean: torch.Tensor | None = None, rstd: torch.Tensor | None = None) -> None:
+    """``y = (x - mean) * rstd * w + b`` per row; ``w`` and ``b`` (``cols`` values, float32 or the rows' type) may be None;
+    ``mean`` and ``rstd`` (float32, ``rows`` values) receive what ``layer_norm_grad`` needs."""
+    t = _type(x, "x")
+    px, ldx = _rows(x, rows, cols, "x", x.dtype)
+    py, ldy = _rows(y, rows, cols, "y", x.dtype)
+    pt = _param_type((w, b), x.dtype)
+    check(_lib.lib().hpcdnn_layer_norm(t, _TYPES[pt], rows, cols, px, ldx, _flat(w, cols, "w", pt), _flat(b, cols, "b", pt), eps, py, ldy,
+                                       _flat(mean, rows, "mean", torch.float32), _flat(rstd, rows, "rstd", torch.float32), _stream()),
+          "hpcdnn_layer_norm")
+
+
+def layer_norm_grad(rows: int, cols: int, dy: torch.Tensor, x: torch.Tensor, w: torch.Tensor | None, mean: torch.Tensor,
+                    rstd: torch.Tensor, dx: torch.Tensor | None, dw: torch.Tensor | None, db: torch.Tensor | None,
+                    ws: torch.Tensor | None = None) -> None:
+    """Gradient of ``layer_norm``: ``dx`` per row and ``dw``, ``db`` summed over the rows, each formed unless None.  ``ws``:
+    scratch of ``layer_norm_grad_workspace_bytes(rows, cols)`` bytes, needed for ``dw`` and ``db``."""
+    t = _type(x, "x")
+    px, ldx = _rows(x, rows, cols, "x", x.dtype)
+    pdy, lddy = _rows(dy, rows, cols, "dy", x.dtype)
+    pdx, lddx = _rows(dx, rows, cols, "dx", x.dtype) if dx is not None else (None, cols)
+    pt = _param_type((w, dw, db), x.dtype)
+    wp, wb = _scratch(ws)
+    check(_lib.lib().hpcdnn_layer_norm_grad(t, _TYPES[pt], rows, cols, pdy, lddy, px, ldx, _flat(w, cols, "w", pt),
+                                            _flat(mean, rows, "mean", torch.float32), _flat(rstd, rows, "rstd", torch.float32), pdx, lddx,
+                                            _flat(dw, cols, "dw", pt), _flat(db, cols, "db", pt), wp, wb, _stream()),
+          "hpcdnn_layer_norm_grad")
+
+
+def layer_norm_grad_workspace_bytes(rows: int, cols: int) -> int:
+    return int(_lib.lib().hpcdnn_workspace_bytes(_lib.OP_LAYER_NORM_GRAD, rows, cols, 0))
+
+
+def w4_gemv(batch: int, M: int, N: int, group: int, alpha: float, q: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None,
+            x: torch.Tensor, beta: float, y: torch.Tensor) -> None:
+    """``y = alpha * x @ W.T + beta * y`` for a few rows of ``x`` (``batch`` x N) and an M x N matrix of 4-bit weights
+    ``W = (q - zeros) * scales``: ``q`` is uint8 with two columns a byte (the even one in the low half) and a row stride
+    that is a multiple of 4; ``scales`` (of x's type) and ``zeros`` (uint8; None: 8) are M x ceil(N / group) with one row
+    stride.  ``sgemv`` is the same product with FP32 weights."""
+    t = _type(x, "x")
+    groups = -(-N // group) if group in W4_GROUPS else 0
+    pq, ldq = _rows(q, M, (N + 1) // 2, "q", torch.uint8)
+    ps, ldg = _rows(scales, M, groups, "scales", x.dtype)
+    pz = None
+    if zeros is not None:
+        pz, ldz = _rows(zeros, M, groups, "zeros", torch.uint8)
+        if M > 1 and ldz != ldg:
+            raise HpcdnnError("scales and zeros must have the same row stride")
+    px, ldx = _rows(x, batch, N, "x", x.dtype)
+    py, ldy = _rows(y, batch, M, "y", x.dtype)
+    if M == 1:  # the stride of a single row says nothing
+        ldq = -(-ldq // 4) * 4
+    check(_lib.lib().hpcdnn_w4_gemv(t, batch, M, N, group, alpha, pq, ldq, ps, pz, ldg, px, ldx, beta, py, ldy, _stream()), "hpcdnn_w4_gemv")
+
+
+def w4_quantize(M: int, N: int, group: int, W: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None) -> None:
+    """Packs a float32 matrix for ``w4_gemv``, all on CPU tensors: symmetric, or with zero points where ``zeros`` is given."""
+    tensors = [("W", W, torch.float32, N), ("q", q, torch.uint8, (N + 1) // 2)]
+    groups = -(-N // group) if group in W4_GROUPS else 0
+    t = _type(scales, "scales")
+    tensors += [("scales", scales, scales.dtype, groups)] + ([("zeros", zeros, torch.uint8, groups)] if zeros is not None else [])
+    for name, v, dtype, cols in tensors:
+        if not (isinstance(v, torch.Tensor) and v.device.type == "cpu" and v.dtype == dtype and v.dim() == 2 and v.shape[0] >= M
+                and v.shape[1] >= cols and (v.shape[1] <= 1 or v.stride(1) == 1)):
+            raise HpcdnnError(f"{name} must be a {dtype} CPU tensor of at least {M}x{cols} elements with contiguous columns")
+    if zeros is not None and M > 1 and zeros.stride(0) != scales.stride(0):
+        raise HpcdnnError("scales and zeros must have the same row stride")
+    ld = [v.stride(0) if v.shape[0] > 1 else max(v.shape[1], 1) for v in (W, q, scales)]
+    check(_lib.lib().hpcdnn_w4_quantize(t, M, N, group, W.data_ptr(), ld[0], q.data_ptr(), ld[1], scales.data_ptr(),
+                                        zeros.data_ptr() if zeros is not None else None, ld[2]), "hpcdnn_w4_quantize")
+
+
+def expert_sort(tokens: int, topk: int, experts: int, ids: torch.Tensor, offsets: torch.Tensor, pos: torch.Tensor,
+                order: torch.Tensor | None = None, ws: torch.Tensor | None = None) -> None:
+    """Sorts the choices ``ids`` (int32, ``tokens`` x ``topk``; outside 0 .. experts-1: sent nowhere) by expert, stably:
+    ``offsets`` (experts + 1) first places, ``pos`` (tokens x topk) the place of every choice or -1, ``order`` the choice at
+    every place.  ``ws``: scratch of ``expert_sort_workspace_bytes(tokens, topk, experts)`` bytes."""
+    pi, ldi = _rows(ids, tokens, topk, "ids", torch.int32)
+    wp, wb = _scratch(ws)
+    check(_lib.lib().hpcdnn_expert_sort(tokens, topk, experts, pi, ldi, _flat(offsets, experts + 1, "offsets", torch.int32),
+                                        _flat(pos, tokens * topk, "pos", torch.int32), _flat(order, tokens * topk, "order", torch.int32),
+                                        wp, wb, _stream()), "hpcdnn_expert_sort")
+
+
+def expert_sort_workspace_bytes(tokens: int, topk: int, experts: int) -> int:
+    return int(_lib.lib().hpcdnn_workspace_bytes(_lib.OP_EXPERT_SORT, tokens, topk, experts))
+
+
+def expert_gather(tokens: int, topk: int, rows: int, cols: int, x: torch.Tensor, pos: torch.Tensor, out: torch.Tensor) -> None:
+    """``out[pos[t][j]] = x[t]``; rows of ``out`` (``rows`` of them) that no choice has stay as they were."""
+    t = _type(x, "x")
+    px, ldx = _rows(x, tokens, cols, "x", x.dtype)
+    po, ldo = _rows(out, rows, cols, "out", x.dtype)
+    check(_lib.lib().hpcdnn_expert_gather(t, tokens, topk, rows, cols, px, ldx, _flat(pos, tokens * topk, "pos", torch.int32), po, ldo,
+                                          _stream()), "hpcdnn_expert_gather")
+
+
+def expert_combine(tokens: int, topk: int, rows: int, cols: int, xs: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor | None,
+                   y: torch.Tensor) -> None:
+    """``y[t] = sum_j weights[t][j] * xs[pos[t][j]]``; with ``weights`` None the plain sum, which is the gradient of
+    ``expert_gather``."""
+    t = _type(xs, "xs")
+    px, ldx = _rows(xs, rows, cols, "xs", xs.dtype)
+    py, ldy = _rows(y, tokens, cols, "y", xs.dtype)
+    check(_lib.lib().hpcdnn_expert_combine(t, tokens, topk, rows, cols, px, ldx, _flat(pos, tokens * topk, "pos", torch.int32),
+                                           _flat(weights, tokens * topk, "weights", torch.float32), py, ldy, _stream()),
+          "hpcdnn_expert_combine")
+
+
+def expert_combine_grad(tokens: int, topk: int, rows: int, cols: int, dy: torch.Tensor, xs: torch.Tensor, pos: torch.Tensor,
+                        weights: torch.Tensor | None, dxs: torch.Tensor | None, dweights: torch.Tensor | None) -> None:
+    """Gradient of ``expert_combine``: ``dxs[pos[t][j]] = weights[t][j] * dy[t]``, ``dweights[t][j] = <dy[t], xs[pos[t][j]]>``;
+    either may be None, rows of ``dxs`` that no choice has stay as they were."""
+    t = _type(dy, "dy")
+    pdy, lddy = _rows(dy, tokens, cols, "dy", dy.dtype)
+    px, ldx = _rows(xs, rows, cols, "xs", dy.dtype) if dweights is not None else (None, cols)
+    pdx, lddx = _rows(dxs, rows, cols, "dxs", dy.dtype) if dxs is not None else (None, cols)
+    check(_lib.lib().hpcdnn_expert_combine_grad(t, tokens, topk, rows, cols, pdy, lddy, px, ldx,
+                                                _flat(pos, tokens * topk, "pos", torch.int32),
+                                                _flat(weights, tokens * topk, "weights", torch.float32), pdx, lddx,
+                                                _flat(dweights, tokens * topk, "dweights", torch.float32), _stream()),
+          "hpcdnn_expert_combine_grad")
+
+
 def fill_uniform(dst: torch.Tensor, seed: int) -> None:
     """Seeded uniform[-1,1) fill of a contiguous vector (device-side generate_random_vector, utils/utils.cu:28-35)."""
     p = _dev(dst, "dst")

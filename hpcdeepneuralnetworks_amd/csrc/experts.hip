@@ -1,0 +1,334 @@
+// Tokens sorted by the expert they are sent to, their rows copied there and summed back with the router's weights, and
+// the gradient of that sum.  With topk choices per token, slot s = t * topk + j is choice j of token t:
+//
+//   sort     stable by expert: pos[s] = place of slot s (-1: sent nowhere), order[pos[s]] = s, offsets[e] = first place of e
+//   gather   out[pos[s]] = x[t]
+//   combine  y[t] = sum_j w[s] xs[pos[s]]                      (with w = 1: the gradient of gather)
+//   gradient dxs[pos[s]] = w[s] dy[t],  dw[s] = <dy[t], xs[pos[s]]>
+//
+// Everything goes token by token, so a token's row is read (or written) once and the topk rows once each: bound by memory.
+#include <algorithm>
+
+#include "layer_types.h"
+
+namespace hpcdnn {
+
+// ---- sort -----------------------------------------------------------------
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortMaxBlocks = 256;
+constexpr int kSortMinSlots = 4096;  // slots of a workgroup; up to this many are sorted by one workgroup in one launch
+
+// Lanes of the wave that hold the same key as this one, among those with `on`: one ballot per bit of the key.
+__device__ __forceinline__ uint64_t same_key(int key, bool on, int bits) {
+    uint64_t m = __ballot(on);
+    for (int b = 0; b < bits; ++b) {
+        const uint64_t one = __ballot((key >> b) & 1);
+        m &= ((key >> b) & 1) ? one : ~one;
+    }
+    return m;
+}
+
+// counts[block][e] = slots of the workgroup's chunk that go to expert e
+__global__ __launch_bounds__(kSortThreads) void expert_count_kernel(int64_t slots, int per_block, int topk, int experts,
+                                                                    const int* __restrict__ ids, int64_t ldids, int* __restrict__ counts) {
+    extern __shared__ int hist[];  // [experts]
+    for (int e = threadIdx.x; e < experts; e += kSortThreads) hist[e] = 0;
+    __syncthreads();
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block, last = min(slots, first + per_block);
+    for (int64_t s = first + threadIdx.x; s < last; s += kSortThreads) {
+        const int t = static_cast<int>(s / topk);
+        const int id = ids[t * ldids + (s - static_cast<int64_t>(t) * topk)];
+        if (id >= 0 && id < experts) atomicAdd(&hist[id], 1);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < experts; e += kSortThreads) counts[static_cast<int64_t>(blockIdx.x) * experts + e] = hist[e];
+}
+
+// Places of the workgroup's slots.  Every workgroup adds up the counts of all workgroups by itself (they come from L2), so
+// there is no launch for a scan; counts == nullptr: one workgroup has all the slots.  Within the workgroup each wave has a
+// run of consecutive slots: it counts them per expert, the counts are scanned over waves, and in a second walk a slot's
+// place is the wave's next place for its expert plus the number of earlier lanes with the same expert.
+__global__ __launch_bounds__(kSortThreads) void expert_place_kernel(int64_t slots, int per_block, int topk, int experts, int bits,
+                                                                    const int* __restrict__ ids, int64_t ldids,
+                                                                    const int* __restrict__ counts, int blocks, int* __restrict__ offsets,
+                                                                    int* __restrict__ pos, int* __restrict__ order) {
+    extern __shared__ int lds[];
+    const int waves = kSortThreads / kWave;
+    int* next = lds;                          // [waves][experts] counts, then next places
+    int* before = lds + waves * experts;      // [experts] slots of earlier workgroups
+    int* total = before + experts;            // [experts] slots of all workgroups, then first places
+    __shared__ int wave_total[kSortThreads / kWave];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    for (int i = threadIdx.x; i < (waves + 2) * experts; i += kSortThreads) lds[i] = 0;
+    __syncthreads();
+
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block, last = min(slots, first + per_block);
+    const int per_wave = per_block / waves;  // a multiple of 64
+    const int64_t begin = first + static_cast<int64_t>(wave) * per_wave, end = min(last, begin + per_wave);
+    auto key_of = [&](int64_t s) {
+        const int t = static_cast<int>(s / topk);
+        return ids[t * ldids + (s - static_cast<int64_t>(t) * topk)];
+    };
+    for (int64_t s = begin + lane; s < end; s += kWave) {
+        const int id = key_of(s);
+        if (id >= 0 && id < experts) atomicAdd(&next[wave * experts + id], 1);
+    }
+    // earlier workgroups' and all workgroups' slots per expert: threads (expert, share of the workgroups)
+    if (counts != nullptr)
+        for (int64_t i = threadIdx.x; i < static_cast<int64_t>(blocks) * experts; i += kSortThreads) {
+            const int e = static_cast<int>(i % experts), c = counts[i];
+            if (c != 0) {
+                if (i / experts < static_cast<int64_t>(blockIdx.x)) atomicAdd(&before[e], c);
+                atomicAdd(&total[e], c);
+            }
+        }
+    __syncthreads();
+    // exclusive scan of the totals over the experts (at most one per thread), and of the waves' counts
+    const int e = threadIdx.x;
+    int mine = 0;
+    if (e < experts) {
+        int sum = 0;
+        for (int w = 0; w < waves; ++w) sum += next[w * experts + e];
+        mine = counts != nullptr ? total[e] : sum;
+    }
+    int scan = mine;
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) {
+        const int v = __shfl_up(scan, d);
+        if (lane >= d) scan += v;
+    }
+    if (lane == kWave - 1) wave_total[wave] = scan;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) scan += wave_total[w];
+    if (e < experts) {
+        int place = scan - mine + before[e];
+        for (int w = 0; w < waves; ++w) {
+            const int n = next[w * experts + e];
+            next[w * experts + e] = place;
+            place += n;
+        }
+        if (blockIdx.x == 0) {
+            offsets[e] = scan - mine;
+            if (e == experts - 1) offsets[experts] = scan;
+        }
+    }
+    __syncthreads();
+    for (int64_t s0 = begin; s0 < end; s0 += kWave) {
+        const int64_t s = s0 + lane;
+        const int id = s < end ? key_of(s) : -1;
+        const bool sent = id >= 0 && id < experts;
+        const uint64_t peers = same_key(id, sent, bits);
+        const int rank = __popcll(peers & ((1ull << lane) - 1));
+        int place = -1;
+        if (sent) place = next[wave * experts + id] + rank;
+        __builtin_amdgcn_wave_barrier();  // all lanes have read their place before the leaders move it on
+        if (sent && rank == 0) next[wave * experts + id] = place + __popcll(peers);
+        __builtin_amdgcn_wave_barrier();
+        if (s < end) pos[s] = place;
+        if (sent && order != nullptr) order[place] = static_cast<int>(s);
+    }
+}
+
+// ---- rows to their places and back ------------------------------------------
+
+constexpr int kRowThreads = 256;
+
+// out[pos[t][j]] = x[t], one workgroup per token and strip of kRowThreads vectors.
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void expert_gather_kernel(int tokens, int topk, int rows, int cols, const T* __restrict__ x,
+                                                                    int64_t ldx, const int* __restrict__ pos, T* __restrict__ out,
+                                                                    int64_t ldout) {
+    const int col = (blockIdx.y * kRowThreads + threadIdx.x) * kVec<T>;
+    for (int t = blockIdx.x; t < tokens; t += gridDim.x) {
+        const v4u v = load_row(x + t * ldx, col, cols);
+        for (int j = 0; j < topk; ++j) {
+            const int p = pos[static_cast<int64_t>(t) * topk + j];
+            if (p >= 0 && p < rows) store_row(out + p * ldout, col, cols, v);
+        }
+    }
+}
+
+// y[t] = sum_j w[t][j] xs[pos[t][j]], added in FP32 in the order of j.
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void expert_combine_kernel(int tokens, int topk, int rows, int cols, const T* __restrict__ xs,
+                                                                     int64_t ldxs, const int* __restrict__ pos,
+                                                                     const float* __restrict__ weights, T* __restrict__ y, int64_t ldy) {
+    const int col = (blockIdx.y * kRowThreads + threadIdx.x) * kVec<T>;
+    for (int t = blockIdx.x; t < tokens; t += gridDim.x) {
+        float acc[kVec<T>];
+#pragma unroll
+        for (int i = 0; i < kVec<T>; ++i) acc[i] = 0.f;
+        for (int j = 0; j < topk; ++j) {
+            const int64_t s = static_cast<int64_t>(t) * topk + j;
+            const int p = pos[s];
+            if (p >= 0 && p < rows) {
+                const float w = weights != nullptr ? weights[s] : 1.f;
+                float f[kVec<T>];
+                unpack<T>(load_row(xs + p * ldxs, col, cols), f);
+#pragma unroll
+                for (int i = 0; i < kVec<T>; ++i) acc[i] = __builtin_fmaf(w, f[i], acc[i]);
+            }
+        }
+        store_row(y + t * ldy, col, cols, pack<T>(acc));
+    }
+}
+
+// dxs[pos[t][j]] = w[t][j] dy[t],  dw[t][j] = <dy[t], xs[pos[t][j]]>: one workgroup per token; a choice's dot product is
+// added over the thread's columns, the lanes and the waves in that fixed order.
+template <class T>
+__global__ __launch_bounds__(kRowThreads) void expert_combine_grad_kernel(int tokens, int topk, int rows, int cols,
+                                                                          const T* __restrict__ dy, int64_t lddy,
+                                                                          const T* __restrict__ xs, int64_t ldxs,
+                                                                          const int* __restrict__ pos, const float* __restrict__ weights,
+                                                                          T* __restrict__ dxs, int64_t lddxs, float* __restrict__ dweights) {
+    constexpr int kWaves = kRowThreads / kWave;
+    __shared__ float part[2][kWaves];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    int turn = 0;
+    for (int t = blockIdx.x; t < tokens; t += gridDim.x)
+        for (int j = 0; j < topk; ++j, turn ^= 1) {
+            const int64_t s = static_cast<int64_t>(t) * topk + j;
+            const int p = pos[s];
+            const bool sent = p >= 0 && p < rows;
+            float dot = 0.f;
+            if (sent) {
+                const float w = weights != nullptr ? weights[s] : 1.f;
+                for (int col = threadIdx.x * kVec<T>; col < cols; col += kRowThreads * kVec<T>) {
+                    float g[kVec<T>], f[kVec<T>];
+                    unpack<T>(load_row(dy + t * lddy, col, cols), g);
+                    if (dweights != nullptr) {
+                        unpack<T>(load_row(xs + p * ldxs, col, cols), f);
+#pragma unroll
+                        for (int i = 0; i < kVec<T>; ++i) dot = __builtin_fmaf(g[i], f[i], dot);
+                    }
+                    if (dxs != nullptr) {
+#pragma unroll
+                        for (int i = 0; i < kVec<T>; ++i) g[i] *= w;
+                        store_row(dxs + p * lddxs, col, cols, pack<T>(g));
+                    }
+                }
+            }
+            if (dweights != nullptr) {
+                dot = wave_allsum(dot);
+                if (lane == 0) part[turn][wave] = dot;
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    float sum = part[turn][0];
+                    for (int w = 1; w < kWaves; ++w) sum += part[turn][w];
+                    dweights[s] = sent ? sum : 0.f;
+                }
+            }
+        }
+}
+
+namespace {
+
+struct sort_plan {
+    int blocks, per_block;
+};
+// Workgroups of kSortMinSlots slots, of more when that would be more than kSortMaxBlocks (every workgroup reads all counts).
+sort_plan plan_sort(int64_t slots) {
+    const int64_t unit = kSortThreads;
+    int64_t per = std::max<int64_t>(kSortMinSlots, ceil_div(ceil_div(slots, kSortMaxBlocks), unit) * unit);
+    return {static_cast<int>(std::max<int64_t>(1, ceil_div(slots, per))), static_cast<int>(per)};
+}
+
+bool choices_valid(int tokens, int topk) {
+    return tokens >= 0 && topk >= 1 && topk <= HPCDNN_EXPERTS_MAX_TOPK && static_cast<int64_t>(tokens) * topk <= INT32_MAX;
+}
+bool rows_valid(const void* p, int64_t ld, int cols, int type) { return p != nullptr && ld >= cols && aligned(p, type_bytes(type)); }
+
+// Workgroups over the tokens: one each up to a limit far above what the chip holds at a time.
+int token_grid(int tokens) { return std::min(tokens, 1 << 20); }
+
+}  // namespace
+
+size_t expert_sort_workspace_bytes(int tokens, int topk, int experts) {
+    if (!choices_valid(tokens, topk) || experts < 1 || experts > HPCDNN_EXPERTS_MAX) return 0;
+    const sort_plan p = plan_sort(static_cast<int64_t>(tokens) * topk);
+    return p.blocks > 1 ? static_cast<size_t>(p.blocks) * experts * sizeof(int) : 0;
+}
+
+}  // namespace hpcdnn
+
+extern "C" int hpcdnn_expert_sort(int tokens, int topk, int experts, const int32_t* ids, int64_t ldids, int32_t* offsets, int32_t* pos,
+                                  int32_t* order, void* ws, size_t ws_bytes, void* stream_) {
+    using namespace hpcdnn;
+    if (!choices_valid(tokens, topk) || experts < 1 || experts > HPCDNN_EXPERTS_MAX || offsets == nullptr || !aligned(offsets, 4))
+        return HPCDNN_ERR_INVALID_VALUE;
+    if (tokens > 0 && (ids == nullptr || ldids < topk || pos == nullptr || !aligned(ids, 4) || !aligned(pos, 4) || !aligned(order, 4)))
+        return HPCDNN_ERR_INVALID_VALUE;
+    const int64_t slots = static_cast<int64_t>(tokens) * topk;
+    const sort_plan p = plan_sort(slots);
+    if (p.blocks > 1) {
+        if (!aligned(ws, 16)) return HPCDNN_ERR_INVALID_VALUE;
+        if (ws == nullptr || ws_bytes < expert_sort_workspace_bytes(tokens, topk, experts)) return HPCDNN_ERR_WORKSPACE;
+    }
+    hipStream_t stream = static_cast<hipStream_t>(stream_);
+    int bits = 0;
+    while ((1 << bits) < experts) ++bits;
+    const size_t lds = static_cast<size_t>(kSortThreads / kWave + 2) * experts * sizeof(int);
+    int* counts = nullptr;
+    if (p.blocks > 1) {
+        counts = static_cast<int*>(ws);
+        expert_count_kernel<<<p.blocks, kSortThreads, experts * sizeof(int), stream>>>(slots, p.per_block, topk, experts, ids, ldids, counts);
+    }
+    expert_place_kernel<<<p.blocks, kSortThreads, lds, stream>>>(slots, p.per_block, topk, experts, bits, ids, ldids, counts, p.blocks,
+                                                                 offsets, pos, order);
+    return launch_status();
+}
+
+extern "C" int hpcdnn_expert_gather(int type, int tokens, int topk, int rows, int cols, const void* x, int64_t ldx, const int32_t* pos,
+                                    void* out, int64_t ldout, void* stream) {
+    using namespace hpcdnn;
+    if (!type_valid(type) || !choices_valid(tokens, topk) || rows < 0 || cols < 0) return HPCDNN_ERR_INVALID_VALUE;
+    if (tokens == 0 || rows == 0 || cols == 0) return HPCDNN_OK;
+    if (!rows_valid(x, ldx, cols, type) || !rows_valid(out, ldout, cols, type) || pos == nullptr || !aligned(pos, 4))
+        return HPCDNN_ERR_INVALID_VALUE;
+    return with_type(type, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        const dim3 grid(token_grid(tokens), static_cast<unsigned>(ceil_div(cols, kRowThreads * kVec<T>)));
+        if (grid.y > 65535) return HPCDNN_ERR_INVALID_VALUE;
+        expert_gather_kernel<T><<<grid, kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
+            tokens, topk, rows, cols, static_cast<const T*>(x), ldx, pos, static_cast<T*>(out), ldout);
+        return launch_status();
+    });
+}
+
+extern "C" int hpcdnn_expert_combine(int type, int tokens, int topk, int rows, int cols, const void* xs, int64_t ldxs, const int32_t* pos,
+                                     const float* weights, void* y, int64_t ldy, void* stream) {
+    using namespace hpcdnn;
+    if (!type_valid(type) || !choices_valid(tokens, topk) || rows < 0 || cols < 0) return HPCDNN_ERR_INVALID_VALUE;
+    if (tokens == 0 || cols == 0) return HPCDNN_OK;
+    if ((rows > 0 && !rows_valid(xs, ldxs, cols, type)) || !rows_valid(y, ldy, cols, type) || pos == nullptr || !aligned(pos, 4) ||
+        !aligned(weights, 4))
+        return HPCDNN_ERR_INVALID_VALUE;
+    return with_type(type, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        const dim3 grid(token_grid(tokens), static_cast<unsigned>(ceil_div(cols, kRowThreads * kVec<T>)));
+        if (grid.y > 65535) return HPCDNN_ERR_INVALID_VALUE;
+        expert_combine_kernel<T><<<grid, kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
+            tokens, topk, rows, cols, static_cast<const T*>(xs), ldxs, pos, weights, static_cast<T*>(y), ldy);
+        return launch_status();
+    });
+}
+
+extern "C" int hpcdnn_expert_combine_grad(int type, int tokens, int topk, int rows, int cols, const void* dy, int64_t lddy, const void* xs,
+                                          int64_t ldxs, const int32_t* pos, const float* weights, void* dxs, int64_t lddxs,
+                                          float* dweights, void* stream) {
+    using namespace hpcdnn;
+    if (!type_valid(type) || !choices_valid(tokens, topk) || rows < 0 || cols < 0) return HPCDNN_ERR_INVALID_VALUE;
+    if (tokens == 0 || (dxs == nullptr && dweights == nullptr)) return HPCDNN_OK;
+    if (pos == nullptr || !aligned(pos, 4) || !aligned(weights, 4) || !aligned(dweights, 4)) return HPCDNN_ERR_INVALID_VALUE;
+    if (cols > 0 && (!rows_valid(dy, lddy, cols, type) || (rows > 0 && dweights && !rows_valid(xs, ldxs, cols, type)) ||
+                     (rows > 0 && dxs && !rows_valid(dxs, lddxs, cols, type))))
+        return HPCDNN_ERR_INVALID_VALUE;
+    return with_type(type, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        expert_combine_grad_kernel<T><<<token_grid(tokens), kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
+            tokens, topk, rows, cols, static_cast<const T*>(dy), lddy, static_cast<const T*>(xs), ldxs, pos, weights,
+            static_cast<T*>(dxs), lddxs, dweights);
+        return launch_status();
+    });
+}

@@ -11,6 +11,8 @@ size_t ft_workspace_bytes(int M, int N, int K);
 size_t ft_cm_nt_workspace_bytes(int M, int N, int K);
 size_t sgemv_workspace_bytes(int M, int N);
 size_t offline_ft_workspace_bytes(int M, int N, int K);
+size_t layer_norm_grad_workspace_bytes(int rows, int cols);
+size_t expert_sort_workspace_bytes(int tokens, int topk, int experts);
 }  // namespace hpcdnn
 
 extern "C" const char* hpcdnn_version(void) { return "hpcdnn 0.1 (gfx950)"; }
@@ -33,6 +35,8 @@ extern "C" size_t hpcdnn_workspace_bytes(int op, int M, int N, int K) {
         case HPCDNN_OP_FT_SGEMM_CM_NT: return hpcdnn::ft_cm_nt_workspace_bytes(M, N, K);
         case HPCDNN_OP_SGEMV: return hpcdnn::sgemv_workspace_bytes(M, N);
         case HPCDNN_OP_OFFLINE_FT_SGEMM: return hpcdnn::offline_ft_workspace_bytes(M, N, K);
+        case HPCDNN_OP_LAYER_NORM_GRAD: return hpcdnn::layer_norm_grad_workspace_bytes(M, N);
+        case HPCDNN_OP_EXPERT_SORT: return hpcdnn::expert_sort_workspace_bytes(M, N, K);
         default: return 0;
     }
 }

@@ -1,0 +1,403 @@
+// Layer normalisation over the rows of a row-major matrix, and its gradient.
+//
+//   mu = sum_c x / C,  var = sum_c (x - mu)^2 / C,  r = 1 / sqrt(var + eps),  y = (x - mu) r w + b
+//   xh = (x - mu) r,   g = dy w,   dx = r (g - sum_c g / C - xh sum_c (g xh) / C),   dw = sum_rows dy xh,   db = sum_rows dy
+//
+// Both are bound by memory: 2 (forward) and 3 (gradient) values moved per element against about 10 operations.  A row
+// is read once and stays in registers between its statistics and its result; all sums are FP32.
+#include <algorithm>
+
+#include "layer_types.h"
+
+namespace hpcdnn {
+
+constexpr int kNormRowWaves = 4;     // rows per workgroup where a wave takes a row of its own
+constexpr int kNormMaxWaves = 16;
+
+// Columns of the calling thread: vector v starts at column (v * team + lane_in_team) * kVec.
+template <class T, int NV>
+struct row_slice {
+    int col[NV];
+    __device__ row_slice(int t, int team) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) col[v] = (v * team + t) * kVec<T>;
+    }
+    __device__ void load(const T* row, int cols, v4u (&u)[NV]) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) u[v] = load_row(row, col[v], cols);
+    }
+};
+
+// Parameters of the thread's columns in FP32; `fill` where there are none (and behind the last column).
+template <class T, class W, int NV>
+__device__ __forceinline__ void load_params(const W* p, float fill, const row_slice<T, NV>& s, int cols, float (&out)[NV][kVec<T>]) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < kVec<T>; ++i)
+            out[v][i] = (p != nullptr && s.col[v] + i < cols) ? static_cast<float>(p[s.col[v] + i]) : fill;
+}
+
+// One row per wave (kWaveRow: no exchange between waves) or per workgroup.  The mean and the squared deviations of a
+// wave's part of the row are formed in two passes over registers, the parts then joined exactly,
+//   mu = sum n_w mu_w / C,   M2 = sum M2_w + n_w (mu_w - mu)^2,
+// so nothing cancels (sum x^2 - C mu^2 would lose the variance of rows with a large mean) and a row costs one barrier.
+// The next row of the workgroup is loaded before the present one is reduced.
+template <class T, class W, int NV, bool kWaveRow>
+__global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer_norm_kernel(
+    int64_t rows, int cols, const T* __restrict__ x, int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, float eps,
+    T* __restrict__ y, int64_t ldy, float* __restrict__ mean, float* __restrict__ rstd) {
+    __shared__ float part[2][2][kNormMaxWaves];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int waves = blockDim.x / kWave;
+    const int64_t step = kWaveRow ? static_cast<int64_t>(gridDim.x) * kNormRowWaves : gridDim.x;
+    int64_t r = kWaveRow ? static_cast<int64_t>(blockIdx.x) * kNormRowWaves + wave : blockIdx.x;
+    if (r >= rows) return;
+    const row_slice<T, NV> s(kWaveRow ? lane : threadIdx.x, kWaveRow ? kWave : blockDim.x);
+    int valid = 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) valid += max(0, min(kVec<T>, cols - s.col[v]));
+    const float n_wave = wave_allsum(static_cast<float>(valid));
+    const float n_cols = static_cast<float>(cols);
+    // columns of wave (lane & 15): what the join below weighs that wave's mean with
+    float n_of_lane = 0.f;
+    if (!kWaveRow) {
+        if (lane == 0) part[0][0][wave] = n_wave;
+        __syncthreads();
+        n_of_lane = (lane & 15) < waves ? part[0][0][lane & 15] : 0.f;
+        __syncthreads();
+    }
+
+    v4u cur[NV], nxt[NV];
+    s.load(x + r * ldx, cols, cur);
+    float wf[NV][kVec<T>], bf[NV][kVec<T>];
+    load_params<T, W, NV>(w, 1.f, s, cols, wf);
+    load_params<T, W, NV>(b, 0.f, s, cols, bf);
+    for (int turn = 0;; turn ^= 1) {
+        const int64_t next = r + step;
+        if (next < rows) s.load(x + next * ldx, cols, nxt);
+        float f[NV][kVec<T>], sum = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            unpack<T>(cur[v], f[v]);
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i) sum += f[v][i];
+        }
+        // divided, not multiplied by a reciprocal: a row of equal values then has exactly that mean, and no spread
+        float mu = wave_allsum(sum) / fmaxf(n_wave, 1.f), m2 = 0.f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i) {
+                const float d = s.col[v] + i < cols ? f[v][i] - mu : 0.f;
+                m2 = __builtin_fmaf(d, d, m2);
+            }
+        m2 = wave_allsum(m2);
+        if (!kWaveRow) {
+            if (lane == 0) {
+                part[turn][0][wave] = mu;
+                part[turn][1][wave] = m2;
+            }
+            __syncthreads();
+            const bool has = (lane & 15) < waves;
+            const float mu_w = has ? part[turn][0][lane & 15] : 0.f, m2_w = has ? part[turn][1][lane & 15] : 0.f;
+            mu = row16_allsum(n_of_lane * mu_w) / n_cols;
+            m2 = row16_allsum(__builtin_fmaf(n_of_lane * (mu_w - mu), mu_w - mu, m2_w));
+        }
+        const float rs = 1.f / __builtin_sqrtf(m2 / n_cols + eps);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            float o[kVec<T>];
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i) o[i] = __builtin_fmaf((f[v][i] - mu) * rs, wf[v][i], bf[v][i]);
+            store_row(y + r * ldy, s.col[v], cols, pack<T>(o));
+        }
+        if ((kWaveRow ? lane : static_cast<int>(threadIdx.x)) == 0) {
+            if (mean != nullptr) mean[r] = mu;
+            if (rstd != nullptr) rstd[r] = rs;
+        }
+        if (next >= rows) break;
+        r = next;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) cur[v] = nxt[v];
+    }
+}
+
+// Gradient.  A workgroup walks its rows (workgroup, workgroup + grid, ...), adding dy xh and dy of its columns in
+// registers, and writes one partial row of each at the end: [workgroup][2][cols] in the workspace, added in the
+// workgroups' order by layer_norm_params_kernel, so dw and db do not depend on timing.
+template <class T, class W, int NV, bool kWaveRow>
+__global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer_norm_grad_kernel(
+    int64_t rows, int cols, const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, const W* __restrict__ w,
+    const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx, int64_t lddx, float* __restrict__ partial) {
+    __shared__ float part[2][2][kNormMaxWaves];
+    extern __shared__ float joined[];  // kWaveRow: [2][cols], the waves' sums added in wave order
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int waves = blockDim.x / kWave;
+    const int64_t step = kWaveRow ? static_cast<int64_t>(gridDim.x) * kNormRowWaves : gridDim.x;
+    int64_t r = kWaveRow ? static_cast<int64_t>(blockIdx.x) * kNormRowWaves + wave : blockIdx.x;
+    const row_slice<T, NV> s(kWaveRow ? lane : threadIdx.x, kWaveRow ? kWave : blockDim.x);
+    const float inv_cols = 1.f / static_cast<float>(cols);
+    float wf[NV][kVec<T>], dw[NV][kVec<T>], db[NV][kVec<T>];
+    load_params<T, W, NV>(w, 1.f, s, cols, wf);
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < kVec<T>; ++i) dw[v][i] = db[v][i] = 0.f;
+    v4u cx[NV], cd[NV], nx[NV], nd[NV];
+    if (r < rows) {
+        s.load(x + r * ldx, cols, cx);
+        s.load(dy + r * lddy, cols, cd);
+    }
+    for (int turn = 0; r < rows; turn ^= 1) {
+        const int64_t next = r + step;
+        if (next < rows) {
+            s.load(x + next * ldx, cols, nx);
+            s.load(dy + next * lddy, cols, nd);
+        }
+        const float mu = mean[r], rs = rstd[r];
+        float g_sum = 0.f, gx_sum = 0.f;
+        float xh[NV][kVec<T>], g[NV][kVec<T>];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            unpack<T>(cx[v], xh[v]);
+            unpack<T>(cd[v], g[v]);
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i) {
+                xh[v][i] = (xh[v][i] - mu) * rs;
+                dw[v][i] = __builtin_fmaf(g[v][i], xh[v][i], dw[v][i]);
+                db[v][i] += g[v][i];
+                g[v][i] *= wf[v][i];
+                g_sum += g[v][i];
+                gx_sum = __builtin_fmaf(g[v][i], xh[v][i], gx_sum);
+            }
+        }
+        if (dx != nullptr) {
+            g_sum = wave_allsum(g_sum);
+            gx_sum = wave_allsum(gx_sum);
+            if (!kWaveRow) {
+                if (lane == 0) {
+                    part[turn][0][wave] = g_sum;
+                    part[turn][1][wave] = gx_sum;
+                }
+                __syncthreads();
+                const bool has = (lane & 15) < waves;
+                g_sum = row16_allsum(has ? part[turn][0][lane & 15] : 0.f);
+                gx_sum = row16_allsum(has ? part[turn][1][lane & 15] : 0.f);
+            }
+            const float a = g_sum * inv_cols, c = gx_sum * inv_cols;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                float o[kVec<T>];
+#pragma unroll
+                for (int i = 0; i < kVec<T>; ++i) o[i] = rs * (g[v][i] - a - xh[v][i] * c);
+                store_row(dx + r * lddx, s.col[v], cols, pack<T>(o));
+            }
+        }
+        r = next;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            cx[v] = nx[v];
+            cd[v] = nd[v];
+        }
+    }
+    if (partial == nullptr) return;
+    float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * cols;
+    if (kWaveRow) {
+        for (int turn = 0; turn < kNormRowWaves; ++turn) {
+            if (turn == wave) {
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+#pragma unroll
+                    for (int i = 0; i < kVec<T>; ++i) {
+                        const int c = s.col[v] + i;
+                        if (c < cols) {
+                            joined[c] = turn == 0 ? dw[v][i] : joined[c] + dw[v][i];
+                            joined[cols + c] = turn == 0 ? db[v][i] : joined[cols + c] + db[v][i];
+                        }
+                    }
+            }
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < 2 * cols; i += blockDim.x) out[i] = joined[i];
+    } else {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i) {
+                const int c = s.col[v] + i;
+                if (c < cols) {
+                    out[c] = dw[v][i];
+                    out[cols + c] = db[v][i];
+                }
+            }
+    }
+}
+
+// dw[c], db[c] = the partial rows added in order: 32 columns by 8 runs of consecutive partial rows per workgroup, the
+// runs added in order.
+template <class W>
+__global__ __launch_bounds__(256) void layer_norm_params_kernel(int parts, int cols, const float* __restrict__ partial, W* __restrict__ dw,
+                                                                W* __restrict__ db) {
+    __shared__ float run[8][32];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x / 32;
+    const int per = (parts + 7) / 8;
+    const int first = k * per, last = min(parts, first + per);
+    float sum = 0.f;
+    if (c < 2 * cols) {
+        constexpr int kBatch = 8;
+        for (int p = first; p < last; p += kBatch) {
+            float t[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) t[u] = p + u < last ? partial[static_cast<int64_t>(p + u) * 2 * cols + c] : 0.f;
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) sum += t[u];
+        }
+    }
+    run[k][threadIdx.x & 31] = sum;
+    __syncthreads();
+    if (k != 0 || c >= 2 * cols) return;
+#pragma unroll
+    for (int u = 1; u < 8; ++u) sum += run[u][threadIdx.x];
+    if (c < cols) {
+        if (dw != nullptr) dw[c] = static_cast<W>(sum);
+    } else if (db != nullptr) {
+        db[c - cols] = static_cast<W>(sum);
+    }
+}
+
+namespace {
+
+// A row's vectors over the lanes: a wave of its own while two vectors per lane hold it, else one workgroup of up to 1024
+// threads with one, two or four vectors per thread.
+struct norm_shape {
+    bool wave_row;
+    int nv, threads;
+};
+norm_shape shape_of(int cols, int vec) {
+    const int vecs = static_cast<int>(ceil_div(cols, vec));
+    if (vecs <= 2 * kWave) return {true, vecs <= kWave ? 1 : 2, kNormRowWaves * kWave};
+    const int nv = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4;
+    return {false, nv, static_cast<int>(ceil_div(ceil_div(vecs, nv), kWave)) * kWave};
+}
+
+// Most workgroups of the gradient, each of which leaves a partial row of dw and db: a function of the sizes and the CU
+// count alone, so the workspace does not depend on the type.
+int grad_blocks(int rows, int cols) {
+    const int per_cu = cols <= 2048 ? 4 : cols <= 4096 ? 2 : 1;
+    const int most = device_cus() * per_cu;
+    return rows < most ? rows : most;
+}
+
+template <class T, class W>
+int launch_norm(int rows, int cols, const void* x, int64_t ldx, const void* w, const void* b, float eps, void* y, int64_t ldy,
+                float* mean, float* rstd, hipStream_t stream) {
+    const norm_shape s = shape_of(cols, kVec<T>);
+    const int64_t blocks = s.wave_row ? ceil_div(rows, kNormRowWaves) : rows;
+    const int64_t most = static_cast<int64_t>(device_cus()) * (2048 / s.threads);
+    const int grid = static_cast<int>(blocks < most ? blocks : most);
+    auto go = [&](auto nv, auto wave_row) {
+        layer_norm_kernel<T, W, decltype(nv)::value, decltype(wave_row)::value><<<grid, s.threads, 0, stream>>>(
+            rows, cols, static_cast<const T*>(x), ldx, static_cast<const W*>(w), static_cast<const W*>(b), eps, static_cast<T*>(y), ldy,
+            mean, rstd);
+    };
+    using std::integral_constant;
+    if (s.wave_row) {
+        if (s.nv == 1) go(integral_constant<int, 1>{}, std::true_type{});
+        else go(integral_constant<int, 2>{}, std::true_type{});
+    } else if (s.nv == 1) go(integral_constant<int, 1>{}, std::false_type{});
+    else if (s.nv == 2) go(integral_constant<int, 2>{}, std::false_type{});
+    else if constexpr (kVec<T> == 4) go(integral_constant<int, 4>{}, std::false_type{});
+    return launch_status();
+}
+
+template <class T, class W>
+int launch_grad(int rows, int cols, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const float* mean,
+                const float* rstd, void* dx, int64_t lddx, void* dw, void* db, float* partial, hipStream_t stream) {
+    const norm_shape s = shape_of(cols, kVec<T>);
+    int grid = grad_blocks(rows, cols);
+    if (s.wave_row) grid = std::min(grid, static_cast<int>(ceil_div(rows, kNormRowWaves)));
+    if (grid > 0) {
+        const size_t lds = s.wave_row && partial ? 2 * static_cast<size_t>(cols) * sizeof(float) : 0;
+        auto go = [&](auto nv, auto wave_row) {
+            layer_norm_grad_kernel<T, W, decltype(nv)::value, decltype(wave_row)::value><<<grid, s.threads, lds, stream>>>(
+                rows, cols, static_cast<const T*>(dy), lddy, static_cast<const T*>(x), ldx, static_cast<const W*>(w), mean, rstd,
+                static_cast<T*>(dx), lddx, partial);
+        };
+        using std::integral_constant;
+        if (s.wave_row) {
+            if (s.nv == 1) go(integral_constant<int, 1>{}, std::true_type{});
+            else go(integral_constant<int, 2>{}, std::true_type{});
+        } else if (s.nv == 1) go(integral_constant<int, 1>{}, std::false_type{});
+        else if (s.nv == 2) go(integral_constant<int, 2>{}, std::false_type{});
+        else if constexpr (kVec<T> == 4) go(integral_constant<int, 4>{}, std::false_type{});
+        if (int e = launch_status()) return e;
+    }
+    if (partial != nullptr || (grid == 0 && (dw || db)))
+        layer_norm_params_kernel<W><<<static_cast<int>(ceil_div(2 * static_cast<int64_t>(cols), 32)), 256, 0, stream>>>(
+            grid, cols, partial, static_cast<W*>(dw), static_cast<W*>(db));
+    return launch_status();
+}
+
+bool args_valid(int type, int wtype, int rows, int cols) {
+    return type_valid(type) && (wtype == HPCDNN_F32 || wtype == type) && rows >= 0 && cols >= 0 && cols <= HPCDNN_LAYER_NORM_MAX_COLS;
+}
+bool matrix_valid(const void* p, int64_t ld, int cols, int type) { return p != nullptr && ld >= cols && aligned(p, type_bytes(type)); }
+bool params_valid(const void* p, int wtype) { return aligned(p, type_bytes(wtype)); }
+
+// f(T*, W*) with the types of the rows and of the parameters
+template <class F>
+int with_types(int type, int wtype, F&& f) {
+    return with_type(type, [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        if constexpr (!std::is_same_v<T, float>)
+            if (wtype == type) return f(t, t);
+        return f(t, static_cast<float*>(nullptr));
+    });
+}
+
+}  // namespace
+
+size_t layer_norm_grad_workspace_bytes(int rows, int cols) {
+    if (rows <= 0 || cols <= 0) return 0;
+    return static_cast<size_t>(grad_blocks(rows, cols)) * 2 * cols * sizeof(float);
+}
+
+}  // namespace hpcdnn
+
+extern "C" int hpcdnn_layer_norm(int type, int wtype, int rows, int cols, const void* x, int64_t ldx, const void* w, const void* b,
+                                 float eps, void* y, int64_t ldy, float* mean, float* rstd, void* stream) {
+    using namespace hpcdnn;
+    if (!args_valid(type, wtype, rows, cols) || !(eps >= 0.f)) return HPCDNN_ERR_INVALID_VALUE;
+    if (rows == 0 || cols == 0) return HPCDNN_OK;
+    if (!matrix_valid(x, ldx, cols, type) || !matrix_valid(y, ldy, cols, type) || !params_valid(w, wtype) || !params_valid(b, wtype) ||
+        !aligned(mean, 4) || !aligned(rstd, 4))
+        return HPCDNN_ERR_INVALID_VALUE;
+    return with_types(type, wtype, [&](auto* t, auto* p) {
+        return launch_norm<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(p)>>(
+            rows, cols, x, ldx, w, b, eps, y, ldy, mean, rstd, static_cast<hipStream_t>(stream));
+    });
+}
+
+extern "C" int hpcdnn_layer_norm_grad(int type, int wtype, int rows, int cols, const void* dy, int64_t lddy, const void* x,
+                                      int64_t ldx, const void* w, const float* mean, const float* rstd, void* dx, int64_t lddx, void* dw,
+                                      void* db, void* ws, size_t ws_bytes, void* stream) {
+    using namespace hpcdnn;
+    if (!args_valid(type, wtype, rows, cols)) return HPCDNN_ERR_INVALID_VALUE;
+    if (cols == 0 || (dx == nullptr && dw == nullptr && db == nullptr)) return HPCDNN_OK;
+    if (!params_valid(w, wtype) || !params_valid(dw, wtype) || !params_valid(db, wtype)) return HPCDNN_ERR_INVALID_VALUE;
+    const bool params = dw != nullptr || db != nullptr;
+    if (rows > 0) {
+        if (!matrix_valid(dy, lddy, cols, type) || !matrix_valid(x, ldx, cols, type) || (dx && !matrix_valid(dx, lddx, cols, type)) ||
+            mean == nullptr || rstd == nullptr || !aligned(mean, 4) || !aligned(rstd, 4) || !aligned(ws, 16))
+            return HPCDNN_ERR_INVALID_VALUE;
+        if (params && (ws == nullptr || ws_bytes < layer_norm_grad_workspace_bytes(rows, cols))) return HPCDNN_ERR_WORKSPACE;
+    }
+    return with_types(type, wtype, [&](auto* t, auto* p) {
+        return launch_grad<std::remove_pointer_t<decltype(t)>, std::remove_pointer_t<decltype(p)>>(
+            rows, cols, dy, lddy, x, ldx, w, mean, rstd, dx, lddx, dw, db, params && rows > 0 ? static_cast<float*>(ws) : nullptr,
+            static_cast<hipStream_t>(stream));
+    });
+}

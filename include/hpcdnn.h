@@ -51,6 +51,13 @@ extern "C" {
 #define HPCDNN_OP_SGEMV 3            /* M, N as passed to hpcdnn_sgemv; only trans = 1 uses a workspace */
 #define HPCDNN_OP_OFFLINE_FT_SGEMM 4
 #define HPCDNN_OP_FT_SGEMM_CM_NT 5     /* M, N, K as passed to hpcdnn_ft_sgemm_cm_nt */
+#define HPCDNN_OP_LAYER_NORM_GRAD 6    /* M = rows, N = cols */
+#define HPCDNN_OP_EXPERT_SORT 7        /* M = tokens, N = topk, K = experts */
+
+/* Element types of the layer operators (everything above them is FP32). */
+#define HPCDNN_F32 0
+#define HPCDNN_F16 1
+#define HPCDNN_BF16 2
 
 /* K panel of hpcdnn_offline_ft_sgemm (the reference checks every 256 columns,
  * kernel/ft_sgemm/include/baseline_ft_sgemm.cuh:3). */
@@ -453,6 +460,77 @@ int hpcdnn_saxpy(int64_t n, float alpha, const float* x, float* y, void* stream)
  * pre-zeroed atomicAdd target, and the sdot + reduction multi-launch chain
  * (kernel/sdot/sdot.cu:9-67, launches :156,:177-187). */
 int hpcdnn_sdot(int64_t n, const float* x, const float* y, float* out, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- Layer operators: what stands between the matrix products of a transformer layer.
+ * They take FP32, FP16 or BF16 rows (`type`, one of HPCDNN_F32 / _F16 / _BF16); strides count elements, rows
+ * need no more than the alignment of their element.  All sums are formed in FP32, results are rounded to
+ * `type` once, and every sum has a fixed order: the same call gives the same bits on every run.  Outputs must
+ * not overlap inputs.  The reference has no counterpart: its path ends at the products. */
+
+/* Layer normalisation of every row of x (rows x cols):
+ *   mean = sum x / cols,  var = sum (x - mean)^2 / cols,  rstd = 1 / sqrt(var + eps),
+ *   y = (x - mean) * rstd * w + b.
+ * `w`, `b` (cols values of `wtype`, which is HPCDNN_F32 or `type`) may be NULL: 1 and 0.  `mean`, `rstd`
+ * (FP32, `rows` values; what the gradient needs) may be NULL.  cols <= HPCDNN_LAYER_NORM_MAX_COLS. */
+#define HPCDNN_LAYER_NORM_MAX_COLS 16384
+int hpcdnn_layer_norm(int type, int wtype, int rows, int cols, const void* x, int64_t ldx, const void* w, const void* b, float eps,
+                      void* y, int64_t ldy, float* mean, float* rstd, void* stream);
+/* Its gradient.  With xh = (x - mean) * rstd and g = dy * w:
+ *   dx = rstd * (g - sum g / cols - xh * sum (g * xh) / cols),  dw = sum over rows of dy * xh,  db = sum over rows of dy.
+ * Each of `dx` (rows x cols), `dw`, `db` (cols values of `wtype`) may be NULL and is then not formed; all are
+ * overwritten.  With no rows dw and db are zero.  `ws`: hpcdnn_workspace_bytes(HPCDNN_OP_LAYER_NORM_GRAD, rows,
+ * cols, 0) bytes, 16-byte aligned, no initialisation; needed for dw and db only. */
+int hpcdnn_layer_norm_grad(int type, int wtype, int rows, int cols, const void* dy, int64_t lddy, const void* x, int64_t ldx,
+                           const void* w, const float* mean, const float* rstd, void* dx, int64_t lddx, void* dw, void* db, void* ws,
+                           size_t ws_bytes, void* stream);
+
+/* hpcdnn_sgemv (trans = 0) for a matrix of 4-bit weights and one or a few vectors:
+ *   y[t][m] = alpha * sum_n W[m][n] * x[t][n] + beta * y[t][m],   W[m][n] = (q[m][n] - z[m][n / group]) * s[m][n / group],
+ * W is M x N, x is batch x N, y is batch x M.  Row m of `q` holds N values of 0 .. 15, two a byte, the even
+ * column in the low half; `ldq` is its length in bytes, a multiple of 4, and q is 4-byte aligned.  `scales`
+ * (of `type`) and `zeros` (bytes, 0 .. 15; NULL: 8 everywhere) hold ceil(N / group) values per row with row
+ * length `ldg`; group is 32, 64 or 128.  beta == 0 never reads y.  What stands behind column N in the last
+ * byte and group is not used.  batch <= HPCDNN_W4_MAX_BATCH, N <= HPCDNN_W4_MAX_COLS.  The weights enter
+ * exactly, but x must stay a factor of 64 below the largest FP32 number, and an infinity in x gives infinities or NaN. */
+#define HPCDNN_W4_MAX_BATCH 65536
+#define HPCDNN_W4_MAX_COLS (1 << 24)
+int hpcdnn_w4_gemv(int type, int batch, int M, int N, int group, float alpha, const uint8_t* q, int64_t ldq, const void* scales,
+                   const uint8_t* zeros, int64_t ldg, const void* x, int64_t ldx, float beta, void* y, int64_t ldy, void* stream);
+/* Makes such a matrix from FP32 weights, all on HOST pointers.  Symmetric (zeros == NULL): s = max |w| / 7 of the
+ * group, q = 8 + w / s; with zero points: s = (max - min) / 15 of a range that includes 0, z = -min / s, q = z +
+ * w / s; rounded to nearest, ties to even, and kept within 0 .. 15, with s already rounded to `type`.  Weights
+ * or scales that are not finite in `type` return HPCDNN_ERR_INVALID_VALUE. */
+int hpcdnn_w4_quantize(int type, int M, int N, int group, const float* W, int64_t ldw, uint8_t* q, int64_t ldq, void* scales,
+                       uint8_t* zeros, int64_t ldg);
+
+/* Tokens sorted by expert.  ids (tokens x topk, row length ldids) names the expert of every choice; a value
+ * outside 0 .. experts-1 (padding, a dropped choice) sends it nowhere.  Choice j of token t is slot t * topk + j.
+ *   pos[slot]    place of the slot among all slots sorted by expert, equal experts in slot order; -1: sent nowhere
+ *   order[place] the slot at that place (may be NULL; places from offsets[experts] on are left as they were)
+ *   offsets[e]   first place of expert e, e = 0 .. experts
+ * (pos is tokens x topk without gaps.)  `ws`: hpcdnn_workspace_bytes(HPCDNN_OP_EXPERT_SORT, tokens, topk,
+ * experts) bytes (0 for few tokens), 16-byte aligned, no initialisation.
+ * experts <= HPCDNN_EXPERTS_MAX, topk <= HPCDNN_EXPERTS_MAX_TOPK, tokens * topk < 2^31. */
+#define HPCDNN_EXPERTS_MAX 512
+#define HPCDNN_EXPERTS_MAX_TOPK 64
+int hpcdnn_expert_sort(int tokens, int topk, int experts, const int32_t* ids, int64_t ldids, int32_t* offsets, int32_t* pos,
+                       int32_t* order, void* ws, size_t ws_bytes, void* stream);
+/* out[pos[t][j]] = x[t]: the rows of x (tokens x cols) at the places of their choices.  A place outside 0 .. rows-1 is
+ * skipped (rows: the rows of `out`, which may be fewer than there are choices); rows of `out` that no choice has
+ * are left as they were.  No two choices share a place. */
+int hpcdnn_expert_gather(int type, int tokens, int topk, int rows, int cols, const void* x, int64_t ldx, const int32_t* pos, void* out,
+                         int64_t ldout, void* stream);
+/* y[t] = sum_j weights[t][j] * xs[pos[t][j]] (weights: FP32, tokens x topk without gaps; NULL: 1, which makes this the
+ * gradient of hpcdnn_expert_gather).  Choices whose place is outside 0 .. rows-1 add nothing; a token without any
+ * gets zeros. */
+int hpcdnn_expert_combine(int type, int tokens, int topk, int rows, int cols, const void* xs, int64_t ldxs, const int32_t* pos,
+                          const float* weights, void* y, int64_t ldy, void* stream);
+/* The gradient of hpcdnn_expert_combine: dxs[pos[t][j]] = weights[t][j] * dy[t] and dweights[t][j] = sum over the
+ * columns of dy[t] * xs[pos[t][j]] (0 where the choice has no place).  Either output may be NULL; rows of dxs
+ * that no choice has are left as they were.  No two choices share a place. */
+int hpcdnn_expert_combine_grad(int type, int tokens, int topk, int rows, int cols, const void* dy, int64_t lddy, const void* xs,
+                               int64_t ldxs, const int32_t* pos, const float* weights, void* dxs, int64_t lddxs, float* dweights,
+                               void* stream);
 
 /* Scratch size for an operation (SGEMM: split-K partials for the split
  * hpcdnn_sgemm would choose, 0 if none; SDOT: the blocks' tagged partials + the call counter; M,N,K

@@ -1,0 +1,208 @@
+"""CPU-side checks of the layer operators: bad arguments are refused before anything is launched, and the host packing of
+4-bit weights against the same formulas in numpy."""
+import ctypes as C
+import os
+
+import numpy as np
+import pytest
+import torch
+
+INVALID, WORKSPACE = 1, 2
+P = C.c_void_p(0x1000)
+ODD = C.c_void_p(0x1001)
+TYPES = {0: torch.float32, 1: torch.float16, 2: torch.bfloat16}
+
+
+@pytest.fixture(scope="module")
+def L():
+    from hpcdeepneuralnetworks_amd import _lib
+
+    if not os.path.exists(_lib.LIB_PATH):
+        _lib.build()
+    return _lib.lib()
+
+
+def _norm(L, type_=0, wtype=0, rows=4, cols=8, x=P, ldx=8, w=P, b=P, eps=1e-5, y=P, ldy=8, mean=P, rstd=P):
+    return L.hpcdnn_layer_norm(type_, wtype, rows, cols, x, ldx, w, b, eps, y, ldy, mean, rstd, None)
+
+
+@pytest.mark.parametrize("bad", [dict(type_=3), dict(type_=-1), dict(wtype=1), dict(type_=1, wtype=2), dict(rows=-1), dict(cols=-1),
+                                 dict(cols=16385, ldx=16385, ldy=16385), dict(x=None), dict(y=None), dict(ldx=7), dict(ldy=7),
+                                 dict(x=ODD), dict(y=C.c_void_p(0x1002)), dict(w=C.c_void_p(0x1002)), dict(mean=ODD), dict(eps=-1e-5),
+                                 dict(eps=float("nan"))])
+def test_layer_norm_refuses(L, bad):
+    assert _norm(L, **bad) == INVALID
+
+
+def test_empty_layer_norm_is_nothing_to_do(L):
+    assert _norm(L, rows=0, x=None, y=None) == 0
+    assert _norm(L, cols=0, x=None, y=None) == 0
+    assert _grad(L, cols=0, x=None) == 0
+    assert _grad(L, dx=None, dw=None, db=None) == 0
+
+
+def _grad(L, type_=0, wtype=0, rows=4, cols=8, dy=P, lddy=8, x=P, ldx=8, w=P, mean=P, rstd=P, dx=P, lddx=8, dw=P, db=P, ws=P, wsb=1 << 30):
+    return L.hpcdnn_layer_norm_grad(type_, wtype, rows, cols, dy, lddy, x, ldx, w, mean, rstd, dx, lddx, dw, db, ws, wsb, None)
+
+
+@pytest.mark.parametrize("bad", [dict(type_=3), dict(type_=2, wtype=1), dict(rows=-1), dict(cols=16385), dict(dy=None), dict(x=None),
+                                 dict(mean=None), dict(rstd=None), dict(lddy=7), dict(ldx=7), dict(lddx=7), dict(dx=ODD), dict(dw=ODD),
+                                 dict(ws=C.c_void_p(0x1008))])
+def test_layer_norm_grad_refuses(L, bad):
+    assert _grad(L, **bad) == INVALID
+
+
+def test_layer_norm_grad_wants_its_workspace(L):
+    need = L.hpcdnn_workspace_bytes(6, 4, 8, 0)
+    assert need > 0 and need % 4 == 0
+    assert _grad(L, ws=None, wsb=0) == WORKSPACE
+    assert _grad(L, wsb=need - 1) == WORKSPACE
+    assert L.hpcdnn_workspace_bytes(6, 0, 8, 0) == 0 and L.hpcdnn_workspace_bytes(6, 8, 0, 0) == 0
+
+
+def _w4(L, type_=1, batch=2, M=4, N=40, group=32, q=P, ldq=20, s=P, z=P, ldg=2, x=P, ldx=40, y=P, ldy=4):
+    return L.hpcdnn_w4_gemv(type_, batch, M, N, group, 1.0, q, ldq, s, z, ldg, x, ldx, 0.0, y, ldy, None)
+
+
+@pytest.mark.parametrize("bad", [dict(type_=3), dict(batch=-1), dict(batch=65537), dict(M=-1), dict(N=-1), dict(N=(1 << 24) + 1), dict(group=16),
+                                 dict(group=48), dict(group=256), dict(q=None), dict(q=C.c_void_p(0x1002)), dict(ldq=16), dict(ldq=22),
+                                 dict(s=None), dict(s=ODD), dict(ldg=1), dict(x=None), dict(x=ODD), dict(ldx=39), dict(y=None), dict(ldy=3)])
+def test_w4_gemv_refuses(L, bad):
+    assert _w4(L, **bad) == INVALID
+
+
+def test_empty_w4_gemv_is_nothing_to_do(L):
+    assert _w4(L, batch=0, x=None, y=None) == 0
+    assert _w4(L, M=0, q=None, y=None) == 0
+
+
+def _sort(L, tokens=4, topk=2, experts=8, ids=P, ldids=2, offsets=P, pos=P, order=P, ws=None, wsb=0):
+    return L.hpcdnn_expert_sort(tokens, topk, experts, ids, ldids, offsets, pos, order, ws, wsb, None)
+
+
+@pytest.mark.parametrize("bad", [dict(tokens=-1), dict(topk=0), dict(topk=65, ldids=65), dict(experts=0), dict(experts=513), dict(ids=None),
+                                 dict(ldids=1), dict(offsets=None), dict(pos=None), dict(pos=ODD), dict(order=ODD),
+                                 dict(tokens=1 << 30, topk=2)])
+def test_expert_sort_refuses(L, bad):
+    assert _sort(L, **bad) == INVALID
+
+
+def test_expert_sort_wants_its_workspace(L):
+    assert L.hpcdnn_workspace_bytes(7, 4, 2, 8) == 0
+    need = L.hpcdnn_workspace_bytes(7, 100000, 8, 64)
+    assert need > 0
+    assert _sort(L, tokens=100000, topk=8, ldids=8, experts=64, ws=None, wsb=0) == WORKSPACE
+    assert _sort(L, tokens=100000, topk=8, ldids=8, experts=64, ws=P, wsb=need - 1) == WORKSPACE
+    assert _sort(L, tokens=100000, topk=8, ldids=8, experts=64, ws=C.c_void_p(0x1004), wsb=need) == INVALID
+
+
+@pytest.mark.parametrize("bad", [dict(type_=5), dict(tokens=-1), dict(topk=0), dict(topk=65), dict(rows=-1), dict(cols=-1), dict(x=None), dict(out=None),
+                                 dict(ldx=7), dict(ldo=7), dict(pos=None), dict(pos=ODD), dict(x=ODD), dict(tokens=1 << 30, topk=4)])
+def test_expert_gather_and_combine_refuse(L, bad):
+    a = dict(type_=1, tokens=4, topk=2, rows=8, cols=8, x=P, ldx=8, pos=P, out=P, ldo=8)
+    a.update(bad)
+    args = (a["type_"], a["tokens"], a["topk"], a["rows"], a["cols"], a["x"], a["ldx"], a["pos"])
+    assert L.hpcdnn_expert_gather(*args, a["out"], a["ldo"], None) == INVALID
+    assert L.hpcdnn_expert_combine(*args, P, a["out"], a["ldo"], None) == INVALID
+
+
+@pytest.mark.parametrize("bad", [dict(type_=5), dict(tokens=-1), dict(topk=0), dict(rows=-1), dict(cols=-1), dict(dy=None), dict(xs=None), dict(lddy=7),
+                                 dict(ldxs=7), dict(lddxs=7), dict(pos=None), dict(dxs=ODD), dict(dw=ODD), dict(w=ODD)])
+def test_expert_combine_grad_refuses(L, bad):
+    a = dict(type_=2, tokens=4, topk=2, rows=8, cols=8, dy=P, lddy=8, xs=P, ldxs=8, pos=P, w=P, dxs=P, lddxs=8, dw=P)
+    a.update(bad)
+    assert L.hpcdnn_expert_combine_grad(*a.values(), None) == INVALID
+
+
+def test_empty_expert_calls_are_nothing_to_do(L):
+    assert L.hpcdnn_expert_gather(0, 0, 2, 8, 8, None, 8, None, None, 8, None) == 0
+    assert L.hpcdnn_expert_gather(0, 4, 2, 0, 8, None, 8, None, None, 8, None) == 0
+    assert L.hpcdnn_expert_combine(0, 0, 2, 8, 8, None, 8, None, None, None, 8, None) == 0
+    assert L.hpcdnn_expert_combine_grad(0, 4, 2, 8, 8, None, 8, None, 8, None, None, None, 8, None, None) == 0
+
+
+# ---- host packing ----------------------------------------------------------
+
+def _pack_numpy(W, group, dtype, zero_points):
+    M, N = W.shape
+    groups = -(-N // group)
+    q = np.zeros((M, N), np.uint8)
+    scales = torch.zeros(M, groups, dtype=dtype)
+    zeros = np.zeros((M, groups), np.uint8)
+    for m in range(M):
+        for g in range(groups):
+            w = W[m, g * group:(g + 1) * group]
+            lo, hi = np.float32(min(w.min(), 0)), np.float32(max(w.max(), 0))
+            s = hi / np.float32(15) - lo / np.float32(15) if zero_points else max(hi, -lo) / np.float32(7)
+            scales[m, g] = float(s)
+            s = np.float32(scales[m, g].float())
+            z = np.float32(8) if not zero_points else np.float32(0) if s == 0 else min(np.float32(15), np.rint(-lo / s))
+            zeros[m, g] = z
+            q[m, g * group:(g + 1) * group] = z if s == 0 else np.clip(np.rint(w / s) + z, 0, 15)
+    return q, scales, zeros
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("zero_points", [False, True])
+@pytest.mark.parametrize("shape", [(3, 32, 32), (5, 129, 64), (2, 1, 128), (4, 257, 128)])
+def test_quantize_matches_the_formula(dtype, zero_points, shape):
+    from hpcdeepneuralnetworks_amd import blas
+
+    M, N, group = shape
+    rng = np.random.default_rng(M * N + group)
+    W = rng.standard_normal((M, N)).astype(np.float32)
+    W[0, : min(N, group)] = 0                      # an empty group: scale 0, every weight 0
+    if N > 1:
+        W[1, -1] = -5.0
+    groups, ldq = -(-N // group), -(-((N + 1) // 2) // 4) * 4
+    q = torch.full((M, ldq), 0xEE, dtype=torch.uint8)
+    scales, zeros = torch.zeros(M, groups, dtype=dtype), torch.zeros(M, groups, dtype=torch.uint8)
+    blas.w4_quantize(M, N, group, torch.from_numpy(W), q, scales, zeros if zero_points else None)
+    rq, rs, rz = _pack_numpy(W, group, dtype, zero_points)
+    low, high = q.numpy() & 15, q.numpy() >> 4
+    both = np.stack([low, high], 2).reshape(M, -1)
+    assert np.array_equal(both[:, :N], rq) and torch.equal(scales, rs)
+    assert np.all(q.numpy()[:, (N + 1) // 2:] == 0xEE)   # bytes behind the row are not touched
+    if zero_points:
+        assert np.array_equal(zeros.numpy(), rz)
+    # half a step of the scale, and where zero points clamp at the range's end one step
+    back = (both[:, :N].astype(np.float32) - (np.repeat(rz, group, 1)[:, :N] if zero_points else 8)) * np.repeat(rs.float().numpy(), group, 1)[:, :N]
+    step = np.repeat(rs.float().numpy(), group, 1)[:, :N]
+    assert np.all(np.abs(back - W) <= step * (1.0 + 8 * torch.finfo(dtype).eps) + 1e-30)
+
+
+def test_quantize_refuses():
+    from hpcdeepneuralnetworks_amd import blas
+
+    W, q, s = torch.randn(2, 64), torch.zeros(2, 32, dtype=torch.uint8), torch.zeros(2, 2)
+    blas.w4_quantize(2, 64, 32, W, q, s)
+    for bad in (float("nan"), float("inf")):
+        V = W.clone()
+        V[1, 3] = bad
+        with pytest.raises(blas.HpcdnnError, match="invalid"):
+            blas.w4_quantize(2, 64, 32, V, q, s)
+    with pytest.raises(blas.HpcdnnError, match="invalid"):
+        blas.w4_quantize(2, 64, 32, W * 1e6, q, s.half())    # the scale leaves the range of FP16
+    with pytest.raises(blas.HpcdnnError):
+        blas.w4_quantize(2, 64, 32, W.double(), q, s)
+    with pytest.raises(blas.HpcdnnError):
+        blas.w4_quantize(2, 64, 32, W, q[:, :31], s)
+    with pytest.raises(blas.HpcdnnError, match="invalid"):
+        blas.w4_quantize(2, 64, 48, W, q, s)
+
+
+def test_wrappers_refuse_host_tensors_and_mixed_types():
+    from hpcdeepneuralnetworks_amd import blas
+
+    x = torch.zeros(4, 8)
+    with pytest.raises(blas.HpcdnnError):
+        blas.layer_norm(4, 8, x, None, None, 1e-5, torch.zeros(4, 8))
+    with pytest.raises(blas.HpcdnnError):
+        blas.layer_norm(4, 8, x.double(), None, None, 1e-5, x.double())
+    with pytest.raises(blas.HpcdnnError):
+        blas.w4_gemv(1, 4, 8, 32, 1.0, torch.zeros(4, 4, dtype=torch.uint8), torch.zeros(4, 1), None, x, 0.0, x)
+    with pytest.raises(blas.HpcdnnError):
+        blas.expert_sort(4, 2, 8, torch.zeros(4, 2, dtype=torch.int32), x, x)
+    with pytest.raises(blas.HpcdnnError):
+        blas._param_type((torch.zeros(8), torch.zeros(8, dtype=torch.float16)), torch.float16)
+    assert blas._param_type((None, torch.zeros(8)), torch.float16) == torch.float32
