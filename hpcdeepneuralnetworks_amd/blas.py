@@ -369,55 +369,74 @@ EXPERTS_MAX = 512
 EXPERTS_MAX_TOPK = 64
 
 
+# The small calls are short against what a Python call costs, so the checks touch each tensor a few times only: the raw
+# device and stream numbers come from torch's binding (2.5 us less than a Stream object).
+
+def _device(t: torch.Tensor, name: str) -> int:
+    """The current device, after a look at one operand: without a GPU there is none to ask for."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise HpcdnnError(f"{name} must be a tensor on the GPU")
+    return torch._C._cuda_getDevice()
+
+
+def _stream_of(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
 def _type(t: torch.Tensor, name: str) -> int:
-    if not isinstance(t, torch.Tensor) or t.dtype not in _TYPES:
+    code = _TYPES.get(t.dtype) if isinstance(t, torch.Tensor) else None
+    if code is None:
         raise HpcdnnError(f"{name} must be a float32, float16 or bfloat16 tensor")
-    return _TYPES[t.dtype]
+    return code
 
 
-def _on_device(t: torch.Tensor, name: str, dtype: torch.dtype) -> int:
+def _on_device(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int) -> None:
+    if isinstance(t, torch.Tensor) and t.dtype == dtype and t.get_device() == dev:
+        return
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype):
         raise HpcdnnError(f"{name} must be a {dtype} tensor on the GPU")
-    if t.device.index != torch.cuda.current_device():
-        raise HpcdnnError(f"{name} is on {t.device}, which is not the current device")
-    return t.data_ptr()
+    raise HpcdnnError(f"{name} is on {t.device}, which is not the current device")
 
 
-def _rows(t: torch.Tensor, rows: int, cols: int, name: str, dtype: torch.dtype):
+def _rows(t: torch.Tensor, rows: int, cols: int, name: str, dtype: torch.dtype, dev: int):
     """Pointer and row stride of a 2-D tensor with contiguous columns."""
-    ptr = _on_device(t, name, dtype)
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < cols:
-        raise HpcdnnError(f"{name} must be 2-D with at least {rows}x{cols} elements, got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    _on_device(t, name, dtype, dev)
+    shape = t.shape
+    if len(shape) != 2 or shape[0] < rows or shape[1] < cols:
+        raise HpcdnnError(f"{name} must be 2-D with at least {rows}x{cols} elements, got {tuple(shape)}")
+    stride = t.stride()
+    if stride[1] != 1 and shape[1] > 1:
         raise HpcdnnError(f"{name} must have contiguous columns")
-    return ptr, t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    return t.data_ptr(), stride[0] if shape[0] > 1 else max(shape[1], 1)
 
 
-def _flat(t: torch.Tensor | None, n: int, name: str, dtype: torch.dtype):
+def _flat(t: torch.Tensor | None, n: int, name: str, dtype: torch.dtype, dev: int):
     """Pointer of a contiguous tensor of at least n elements, None for None."""
     if t is None:
         return None
-    ptr = _on_device(t, name, dtype)
+    _on_device(t, name, dtype, dev)
     if t.numel() < n or not t.is_contiguous():
         raise HpcdnnError(f"{name} must be contiguous with at least {n} elements")
-    return ptr
+    return t.data_ptr()
 
 
-def _scratch(ws: torch.Tensor | None):
+def _scratch(ws: torch.Tensor | None, dev: int):
     if ws is None:
         return None, 0
-    if not (ws.is_cuda and ws.is_contiguous()) or ws.device.index != torch.cuda.current_device():
+    if not ws.is_contiguous() or ws.get_device() != dev:
         raise HpcdnnError("ws must be a contiguous tensor on the current device")
     return ws.data_ptr(), ws.numel() * ws.element_size()
 
 
 def _param_type(params, dtype: torch.dtype) -> torch.dtype:
-    kinds = {p.dtype for p in params if p is not None}
-    if not kinds:
-        return torch.float32
-    if len(kinds) > 1 or not kinds <= {torch.float32, dtype}:
-        raise HpcdnnError("w, b and their gradients must share one type: float32 or that of the rows")
-    return kinds.pop()
+    kind = None
+    for p in params:
+        if p is not None:
+            if kind is None:
+                kind = p.dtype
+            if p.dtype != kind or (kind != torch.float32 and kind != dtype):
+                raise HpcdnnError("w, b and their gradients must share one type: float32 or that of the rows")
+    return torch.float32 if kind is None else kind
 
 
 def layer_norm(rows: int, cols: int, x: torch.Tensor, w: torch.Tensor | None, b: torch.Tensor | None, eps: float,
@@ -425,11 +444,12 @@ def layer_norm(rows: int, cols: int, x: torch.Tensor, w: torch.Tensor | None, b:
     """``y = (x - mean) * rstd * w + b`` per row; ``w`` and ``b`` (``cols`` values, float32 or the rows' type) may be None;
     ``mean`` and ``rstd`` (float32, ``rows`` values) receive what ``layer_norm_grad`` needs."""
     t = _type(x, "x")
-    px, ldx = _rows(x, rows, cols, "x", x.dtype)
-    py, ldy = _rows(y, rows, cols, "y", x.dtype)
+    dev = _device(x, "x")
+    px, ldx = _rows(x, rows, cols, "x", x.dtype, dev)
+    py, ldy = _rows(y, rows, cols, "y", x.dtype, dev)
     pt = _param_type((w, b), x.dtype)
-    check(_lib.lib().hpcdnn_layer_norm(t, _TYPES[pt], rows, cols, px, ldx, _flat(w, cols, "w", pt), _flat(b, cols, "b", pt), eps, py, ldy,
-                                       _flat(mean, rows, "mean", torch.float32), _flat(rstd, rows, "rstd", torch.float32), _stream()),
+    check(_lib.lib().hpcdnn_layer_norm(t, _TYPES[pt], rows, cols, px, ldx, _flat(w, cols, "w", pt, dev), _flat(b, cols, "b", pt, dev), eps, py, ldy,
+                                       _flat(mean, rows, "mean", torch.float32, dev), _flat(rstd, rows, "rstd", torch.float32, dev), _stream_of(dev)),
           "hpcdnn_layer_norm")
 
 
@@ -439,14 +459,15 @@ def layer_norm_grad(rows: int, cols: int, dy: torch.Tensor, x: torch.Tensor, w: 
     """Gradient of ``layer_norm``: ``dx`` per row and ``dw``, ``db`` summed over the rows, each formed unless None.  ``ws``:
     scratch of ``layer_norm_grad_workspace_bytes(rows, cols)`` bytes, needed for ``dw`` and ``db``."""
     t = _type(x, "x")
-    px, ldx = _rows(x, rows, cols, "x", x.dtype)
-    pdy, lddy = _rows(dy, rows, cols, "dy", x.dtype)
-    pdx, lddx = _rows(dx, rows, cols, "dx", x.dtype) if dx is not None else (None, cols)
+    dev = _device(x, "x")
+    px, ldx = _rows(x, rows, cols, "x", x.dtype, dev)
+    pdy, lddy = _rows(dy, rows, cols, "dy", x.dtype, dev)
+    pdx, lddx = _rows(dx, rows, cols, "dx", x.dtype, dev) if dx is not None else (None, cols)
     pt = _param_type((w, dw, db), x.dtype)
-    wp, wb = _scratch(ws)
-    check(_lib.lib().hpcdnn_layer_norm_grad(t, _TYPES[pt], rows, cols, pdy, lddy, px, ldx, _flat(w, cols, "w", pt),
-                                            _flat(mean, rows, "mean", torch.float32), _flat(rstd, rows, "rstd", torch.float32), pdx, lddx,
-                                            _flat(dw, cols, "dw", pt), _flat(db, cols, "db", pt), wp, wb, _stream()),
+    wp, wb = _scratch(ws, dev)
+    check(_lib.lib().hpcdnn_layer_norm_grad(t, _TYPES[pt], rows, cols, pdy, lddy, px, ldx, _flat(w, cols, "w", pt, dev),
+                                            _flat(mean, rows, "mean", torch.float32, dev), _flat(rstd, rows, "rstd", torch.float32, dev), pdx, lddx,
+                                            _flat(dw, cols, "dw", pt, dev), _flat(db, cols, "db", pt, dev), wp, wb, _stream_of(dev)),
           "hpcdnn_layer_norm_grad")
 
 
@@ -461,26 +482,29 @@ def w4_gemv(batch: int, M: int, N: int, group: int, alpha: float, q: torch.Tenso
     that is a multiple of 4; ``scales`` (of x's type) and ``zeros`` (uint8; None: 8) are M x ceil(N / group) with one row
     stride.  ``sgemv`` is the same product with FP32 weights."""
     t = _type(x, "x")
+    dev = _device(x, "x")
     groups = -(-N // group) if group in W4_GROUPS else 0
-    pq, ldq = _rows(q, M, (N + 1) // 2, "q", torch.uint8)
-    ps, ldg = _rows(scales, M, groups, "scales", x.dtype)
+    pq, ldq = _rows(q, M, (N + 1) // 2, "q", torch.uint8, dev)
+    ps, ldg = _rows(scales, M, groups, "scales", x.dtype, dev)
     pz = None
     if zeros is not None:
-        pz, ldz = _rows(zeros, M, groups, "zeros", torch.uint8)
+        pz, ldz = _rows(zeros, M, groups, "zeros", torch.uint8, dev)
         if M > 1 and ldz != ldg:
             raise HpcdnnError("scales and zeros must have the same row stride")
-    px, ldx = _rows(x, batch, N, "x", x.dtype)
-    py, ldy = _rows(y, batch, M, "y", x.dtype)
+    px, ldx = _rows(x, batch, N, "x", x.dtype, dev)
+    py, ldy = _rows(y, batch, M, "y", x.dtype, dev)
     if M == 1:  # the stride of a single row says nothing
         ldq = -(-ldq // 4) * 4
-    check(_lib.lib().hpcdnn_w4_gemv(t, batch, M, N, group, alpha, pq, ldq, ps, pz, ldg, px, ldx, beta, py, ldy, _stream()), "hpcdnn_w4_gemv")
+    check(_lib.lib().hpcdnn_w4_gemv(t, batch, M, N, group, alpha, pq, ldq, ps, pz, ldg, px, ldx, beta, py, ldy, _stream_of(dev)), "hpcdnn_w4_gemv")
 
 
 def w4_quantize(M: int, N: int, group: int, W: torch.Tensor, q: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None) -> None:
     """Packs a float32 matrix for ``w4_gemv``, all on CPU tensors: symmetric, or with zero points where ``zeros`` is given."""
+    if not isinstance(scales, torch.Tensor):
+        raise HpcdnnError("scales must be a tensor")
     tensors = [("W", W, torch.float32, N), ("q", q, torch.uint8, (N + 1) // 2)]
     groups = -(-N // group) if group in W4_GROUPS else 0
-    t = _type(scales, "scales")
+    t = _TYPES.get(scales.dtype, -1)
     tensors += [("scales", scales, scales.dtype, groups)] + ([("zeros", zeros, torch.uint8, groups)] if zeros is not None else [])
     for name, v, dtype, cols in tensors:
         if not (isinstance(v, torch.Tensor) and v.device.type == "cpu" and v.dtype == dtype and v.dim() == 2 and v.shape[0] >= M
@@ -498,11 +522,12 @@ def expert_sort(tokens: int, topk: int, experts: int, ids: torch.Tensor, offsets
     """Sorts the choices ``ids`` (int32, ``tokens`` x ``topk``; outside 0 .. experts-1: sent nowhere) by expert, stably:
     ``offsets`` (experts + 1) first places, ``pos`` (tokens x topk) the place of every choice or -1, ``order`` the choice at
     every place.  ``ws``: scratch of ``expert_sort_workspace_bytes(tokens, topk, experts)`` bytes."""
-    pi, ldi = _rows(ids, tokens, topk, "ids", torch.int32)
-    wp, wb = _scratch(ws)
-    check(_lib.lib().hpcdnn_expert_sort(tokens, topk, experts, pi, ldi, _flat(offsets, experts + 1, "offsets", torch.int32),
-                                        _flat(pos, tokens * topk, "pos", torch.int32), _flat(order, tokens * topk, "order", torch.int32),
-                                        wp, wb, _stream()), "hpcdnn_expert_sort")
+    dev = _device(ids, "ids")
+    pi, ldi = _rows(ids, tokens, topk, "ids", torch.int32, dev)
+    wp, wb = _scratch(ws, dev)
+    check(_lib.lib().hpcdnn_expert_sort(tokens, topk, experts, pi, ldi, _flat(offsets, experts + 1, "offsets", torch.int32, dev),
+                                        _flat(pos, tokens * topk, "pos", torch.int32, dev), _flat(order, tokens * topk, "order", torch.int32, dev),
+                                        wp, wb, _stream_of(dev)), "hpcdnn_expert_sort")
 
 
 def expert_sort_workspace_bytes(tokens: int, topk: int, experts: int) -> int:
@@ -512,10 +537,11 @@ def expert_sort_workspace_bytes(tokens: int, topk: int, experts: int) -> int:
 def expert_gather(tokens: int, topk: int, rows: int, cols: int, x: torch.Tensor, pos: torch.Tensor, out: torch.Tensor) -> None:
     """``out[pos[t][j]] = x[t]``; rows of ``out`` (``rows`` of them) that no choice has stay as they were."""
     t = _type(x, "x")
-    px, ldx = _rows(x, tokens, cols, "x", x.dtype)
-    po, ldo = _rows(out, rows, cols, "out", x.dtype)
-    check(_lib.lib().hpcdnn_expert_gather(t, tokens, topk, rows, cols, px, ldx, _flat(pos, tokens * topk, "pos", torch.int32), po, ldo,
-                                          _stream()), "hpcdnn_expert_gather")
+    dev = _device(x, "x")
+    px, ldx = _rows(x, tokens, cols, "x", x.dtype, dev)
+    po, ldo = _rows(out, rows, cols, "out", x.dtype, dev)
+    check(_lib.lib().hpcdnn_expert_gather(t, tokens, topk, rows, cols, px, ldx, _flat(pos, tokens * topk, "pos", torch.int32, dev), po, ldo,
+                                          _stream_of(dev)), "hpcdnn_expert_gather")
 
 
 def expert_combine(tokens: int, topk: int, rows: int, cols: int, xs: torch.Tensor, pos: torch.Tensor, weights: torch.Tensor | None,
@@ -523,10 +549,11 @@ def expert_combine(tokens: int, topk: int, rows: int, cols: int, xs: torch.Tenso
     """``y[t] = sum_j weights[t][j] * xs[pos[t][j]]``; with ``weights`` None the plain sum, which is the gradient of
     ``expert_gather``."""
     t = _type(xs, "xs")
-    px, ldx = _rows(xs, rows, cols, "xs", xs.dtype)
-    py, ldy = _rows(y, tokens, cols, "y", xs.dtype)
-    check(_lib.lib().hpcdnn_expert_combine(t, tokens, topk, rows, cols, px, ldx, _flat(pos, tokens * topk, "pos", torch.int32),
-                                           _flat(weights, tokens * topk, "weights", torch.float32), py, ldy, _stream()),
+    dev = _device(xs, "xs")
+    px, ldx = _rows(xs, rows, cols, "xs", xs.dtype, dev)
+    py, ldy = _rows(y, tokens, cols, "y", xs.dtype, dev)
+    check(_lib.lib().hpcdnn_expert_combine(t, tokens, topk, rows, cols, px, ldx, _flat(pos, tokens * topk, "pos", torch.int32, dev),
+                                           _flat(weights, tokens * topk, "weights", torch.float32, dev), py, ldy, _stream_of(dev)),
           "hpcdnn_expert_combine")
 
 
@@ -535,13 +562,14 @@ def expert_combine_grad(tokens: int, topk: int, rows: int, cols: int, dy: torch.
     """Gradient of ``expert_combine``: ``dxs[pos[t][j]] = weights[t][j] * dy[t]``, ``dweights[t][j] = <dy[t], xs[pos[t][j]]>``;
     either may be None, rows of ``dxs`` that no choice has stay as they were."""
     t = _type(dy, "dy")
-    pdy, lddy = _rows(dy, tokens, cols, "dy", dy.dtype)
-    px, ldx = _rows(xs, rows, cols, "xs", dy.dtype) if dweights is not None else (None, cols)
-    pdx, lddx = _rows(dxs, rows, cols, "dxs", dy.dtype) if dxs is not None else (None, cols)
+    dev = _device(dy, "dy")
+    pdy, lddy = _rows(dy, tokens, cols, "dy", dy.dtype, dev)
+    px, ldx = _rows(xs, rows, cols, "xs", dy.dtype, dev) if dweights is not None else (None, cols)
+    pdx, lddx = _rows(dxs, rows, cols, "dxs", dy.dtype, dev) if dxs is not None else (None, cols)
     check(_lib.lib().hpcdnn_expert_combine_grad(t, tokens, topk, rows, cols, pdy, lddy, px, ldx,
-                                                _flat(pos, tokens * topk, "pos", torch.int32),
-                                                _flat(weights, tokens * topk, "weights", torch.float32), pdx, lddx,
-                                                _flat(dweights, tokens * topk, "dweights", torch.float32), _stream()),
+                                                _flat(pos, tokens * topk, "pos", torch.int32, dev),
+                                                _flat(weights, tokens * topk, "weights", torch.float32, dev), pdx, lddx,
+                                                _flat(dweights, tokens * topk, "dweights", torch.float32, dev), _stream_of(dev)),
           "hpcdnn_expert_combine_grad")
 
 
