@@ -135,88 +135,124 @@ __global__ __launch_bounds__(kSortThreads) void expert_place_kernel(int64_t slot
 constexpr int kRowThreads = 256;
 
 // out[pos[t][j]] = x[t], one workgroup per token and strip of kRowThreads vectors.
-template <class T>
+template <class T, bool kDwords>
 __global__ __launch_bounds__(kRowThreads) void expert_gather_kernel(int tokens, int topk, int rows, int cols, const T* __restrict__ x,
                                                                     int64_t ldx, const int* __restrict__ pos, T* __restrict__ out,
                                                                     int64_t ldout) {
-    const int col = (blockIdx.y * kRowThreads + threadIdx.x) * kVec<T>;
+    const int first = blockIdx.y * kRowThreads * kVec<T>, here = min(cols - first, kRowThreads * kVec<T>);
     for (int t = blockIdx.x; t < tokens; t += gridDim.x) {
-        const v4u v = load_row(x + t * ldx, col, cols);
+        row_values<T, 1, kDwords> v(threadIdx.x, kRowThreads);
+        v.load(x + t * ldx + first, here);
         for (int j = 0; j < topk; ++j) {
             const int p = pos[static_cast<int64_t>(t) * topk + j];
-            if (p >= 0 && p < rows) store_row(out + p * ldout, col, cols, v);
+            const bool is = p >= 0 && p < rows;
+            v.copy_to(out + (is ? p : 0) * ldout + first, is ? here : 0);
         }
     }
 }
 
-// y[t] = sum_j w[t][j] xs[pos[t][j]], added in FP32 in the order of j.
-template <class T>
+// y[t] = sum_j w[t][j] xs[pos[t][j]], added in FP32 in the order of j; kBatch rows are on their way at a time.
+template <class T, bool kDwords>
 __global__ __launch_bounds__(kRowThreads) void expert_combine_kernel(int tokens, int topk, int rows, int cols, const T* __restrict__ xs,
                                                                      int64_t ldxs, const int* __restrict__ pos,
                                                                      const float* __restrict__ weights, T* __restrict__ y, int64_t ldy) {
-    const int col = (blockIdx.y * kRowThreads + threadIdx.x) * kVec<T>;
+    constexpr int kBatch = 4;
+    const int first = blockIdx.y * kRowThreads * kVec<T>, here = min(cols - first, kRowThreads * kVec<T>);
     for (int t = blockIdx.x; t < tokens; t += gridDim.x) {
-        float acc[kVec<T>];
+        float acc[1][kVec<T>];
 #pragma unroll
-        for (int i = 0; i < kVec<T>; ++i) acc[i] = 0.f;
-        for (int j = 0; j < topk; ++j) {
-            const int64_t s = static_cast<int64_t>(t) * topk + j;
-            const int p = pos[s];
-            if (p >= 0 && p < rows) {
-                const float w = weights != nullptr ? weights[s] : 1.f;
-                float f[kVec<T>];
-                unpack<T>(load_row(xs + p * ldxs, col, cols), f);
+        for (int i = 0; i < kVec<T>; ++i) acc[0][i] = 0.f;
+        row_values<T, 1, kDwords> sum(threadIdx.x, kRowThreads);
+        for (int j0 = 0; j0 < topk; j0 += kBatch) {
+            row_values<T, 1, kDwords> v[kBatch] = {sum, sum, sum, sum};
+            float w[kBatch];
 #pragma unroll
-                for (int i = 0; i < kVec<T>; ++i) acc[i] = __builtin_fmaf(w, f[i], acc[i]);
+            for (int b = 0; b < kBatch; ++b) {
+                const int j = min(j0 + b, topk - 1);
+                const int64_t s = static_cast<int64_t>(t) * topk + j;
+                const int p = pos[s];
+                const bool is = j0 + b < topk && p >= 0 && p < rows;  // else zeros, which weigh nothing whatever the weight
+                w[b] = !is ? 0.f : weights != nullptr ? weights[s] : 1.f;
+                v[b].load(xs + (is ? p : 0) * ldxs + first, is ? here : 0);
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                float f[1][kVec<T>];
+                v[b].get(f);
+#pragma unroll
+                for (int i = 0; i < kVec<T>; ++i) acc[0][i] = __builtin_fmaf(w[b], f[0][i], acc[0][i]);
             }
         }
-        store_row(y + t * ldy, col, cols, pack<T>(acc));
+        sum.store(y + t * ldy + first, here, acc);
     }
 }
 
 // dxs[pos[t][j]] = w[t][j] dy[t],  dw[t][j] = <dy[t], xs[pos[t][j]]>: one workgroup per token; a choice's dot product is
 // added over the thread's columns, the lanes and the waves in that fixed order.
-template <class T>
+template <class T, bool kDwords>
 __global__ __launch_bounds__(kRowThreads) void expert_combine_grad_kernel(int tokens, int topk, int rows, int cols,
                                                                           const T* __restrict__ dy, int64_t lddy,
                                                                           const T* __restrict__ xs, int64_t ldxs,
                                                                           const int* __restrict__ pos, const float* __restrict__ weights,
                                                                           T* __restrict__ dxs, int64_t lddxs, float* __restrict__ dweights) {
-    constexpr int kWaves = kRowThreads / kWave;
-    __shared__ float part[2][kWaves];
+    constexpr int kWaves = kRowThreads / kWave, kBatch = 2;
+    constexpr int kStrip = kRowThreads * kVec<T>;
+    __shared__ float part[2][kBatch][kWaves];
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     int turn = 0;
     for (int t = blockIdx.x; t < tokens; t += gridDim.x)
-        for (int j = 0; j < topk; ++j, turn ^= 1) {
-            const int64_t s = static_cast<int64_t>(t) * topk + j;
-            const int p = pos[s];
-            const bool sent = p >= 0 && p < rows;
-            float dot = 0.f;
-            if (sent) {
-                const float w = weights != nullptr ? weights[s] : 1.f;
-                for (int col = threadIdx.x * kVec<T>; col < cols; col += kRowThreads * kVec<T>) {
-                    float g[kVec<T>], f[kVec<T>];
-                    unpack<T>(load_row(dy + t * lddy, col, cols), g);
-                    if (dweights != nullptr) {
-                        unpack<T>(load_row(xs + p * ldxs, col, cols), f);
+        for (int j0 = 0; j0 < topk; j0 += kBatch, turn ^= 1) {
+            int p[kBatch];
+            float w[kBatch], dot[kBatch];
+            bool is[kBatch];
 #pragma unroll
-                        for (int i = 0; i < kVec<T>; ++i) dot = __builtin_fmaf(g[i], f[i], dot);
+            for (int b = 0; b < kBatch; ++b) {
+                const int64_t s = static_cast<int64_t>(t) * topk + min(j0 + b, topk - 1);
+                p[b] = pos[s];
+                is[b] = j0 + b < topk && p[b] >= 0 && p[b] < rows;
+                w[b] = !is[b] ? 0.f : weights != nullptr ? weights[s] : 1.f;
+                dot[b] = 0.f;
+            }
+            bool any = false;
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) any |= is[b];
+            if (any)
+                for (int first = 0; first < cols; first += kStrip) {
+                    const int here = min(cols - first, kStrip);
+                    row_values<T, 1, kDwords> g(threadIdx.x, kRowThreads), v[kBatch] = {g, g};
+                    g.load(dy + t * lddy + first, here);
+#pragma unroll
+                    for (int b = 0; b < kBatch; ++b) {
+                        const bool read = is[b] && dweights != nullptr;
+                        v[b].load(xs + (read ? p[b] : 0) * ldxs + first, read ? here : 0);
                     }
-                    if (dxs != nullptr) {
+                    float gf[1][kVec<T>];
+                    g.get(gf);
 #pragma unroll
-                        for (int i = 0; i < kVec<T>; ++i) g[i] *= w;
-                        store_row(dxs + p * lddxs, col, cols, pack<T>(g));
+                    for (int b = 0; b < kBatch; ++b) {
+                        const bool write = is[b] && dxs != nullptr;
+                        float f[1][kVec<T>];
+                        v[b].get(f);
+#pragma unroll
+                        for (int i = 0; i < kVec<T>; ++i) {
+                            dot[b] = __builtin_fmaf(gf[0][i], f[0][i], dot[b]);
+                            f[0][i] = gf[0][i] * w[b];
+                        }
+                        g.store(dxs + (write ? p[b] : 0) * lddxs + first, write ? here : 0, f);
                     }
                 }
-            }
             if (dweights != nullptr) {
-                dot = wave_allsum(dot);
-                if (lane == 0) part[turn][wave] = dot;
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) {
+                    dot[b] = wave_allsum(dot[b]);
+                    if (lane == 0) part[turn][b][wave] = dot[b];
+                }
                 __syncthreads();
-                if (threadIdx.x == 0) {
-                    float sum = part[turn][0];
-                    for (int w = 1; w < kWaves; ++w) sum += part[turn][w];
-                    dweights[s] = sent ? sum : 0.f;
+                const int b = threadIdx.x;
+                if (b < kBatch && j0 + b < topk) {
+                    float sum = part[turn][b][0];
+                    for (int k = 1; k < kWaves; ++k) sum += part[turn][b][k];
+                    dweights[static_cast<int64_t>(t) * topk + j0 + b] = is[b] ? sum : 0.f;
                 }
             }
         }
@@ -238,6 +274,16 @@ bool choices_valid(int tokens, int topk) {
     return tokens >= 0 && topk >= 1 && topk <= HPCDNN_EXPERTS_MAX_TOPK && static_cast<int64_t>(tokens) * topk <= INT32_MAX;
 }
 bool rows_valid(const void* p, int64_t ld, int cols, int type) { return p != nullptr && ld >= cols && aligned(p, type_bytes(type)); }
+
+// f(T*, kDwords) with the type of the rows and whether they can be read 16 bytes at a time
+template <class F>
+int with_rows(int type, bool dwords, F&& f) {
+    return with_type(type, [&](auto* t) {
+        if constexpr (sizeof(*t) == 2)
+            if (!dwords) return f(t, std::false_type{});
+        return f(t, std::true_type{});
+    });
+}
 
 // Workgroups over the tokens: one each up to a limit far above what the chip holds at a time.
 int token_grid(int tokens) { return std::min(tokens, 1 << 20); }
@@ -282,15 +328,15 @@ extern "C" int hpcdnn_expert_sort(int tokens, int topk, int experts, const int32
 extern "C" int hpcdnn_expert_gather(int type, int tokens, int topk, int rows, int cols, const void* x, int64_t ldx, const int32_t* pos,
                                     void* out, int64_t ldout, void* stream) {
     using namespace hpcdnn;
-    if (!type_valid(type) || !choices_valid(tokens, topk) || rows < 0 || cols < 0) return HPCDNN_ERR_INVALID_VALUE;
+    if (!type_valid(type) || !choices_valid(tokens, topk) || rows < 0 || cols < 0 || cols > HPCDNN_EXPERTS_MAX_COLS) return HPCDNN_ERR_INVALID_VALUE;
     if (tokens == 0 || rows == 0 || cols == 0) return HPCDNN_OK;
     if (!rows_valid(x, ldx, cols, type) || !rows_valid(out, ldout, cols, type) || pos == nullptr || !aligned(pos, 4))
         return HPCDNN_ERR_INVALID_VALUE;
-    return with_type(type, [&](auto* t) {
+    const size_t e = type_bytes(type);
+    return with_rows(type, rows_are_dwords(x, ldx, cols, e) && rows_are_dwords(out, ldout, cols, e), [&](auto* t, auto dwords) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
         const dim3 grid(token_grid(tokens), static_cast<unsigned>(ceil_div(cols, kRowThreads * kVec<T>)));
-        if (grid.y > 65535) return HPCDNN_ERR_INVALID_VALUE;
-        expert_gather_kernel<T><<<grid, kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
+        expert_gather_kernel<T, decltype(dwords)::value><<<grid, kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
             tokens, topk, rows, cols, static_cast<const T*>(x), ldx, pos, static_cast<T*>(out), ldout);
         return launch_status();
     });
@@ -299,16 +345,16 @@ extern "C" int hpcdnn_expert_gather(int type, int tokens, int topk, int rows, in
 extern "C" int hpcdnn_expert_combine(int type, int tokens, int topk, int rows, int cols, const void* xs, int64_t ldxs, const int32_t* pos,
                                      const float* weights, void* y, int64_t ldy, void* stream) {
     using namespace hpcdnn;
-    if (!type_valid(type) || !choices_valid(tokens, topk) || rows < 0 || cols < 0) return HPCDNN_ERR_INVALID_VALUE;
+    if (!type_valid(type) || !choices_valid(tokens, topk) || rows < 0 || cols < 0 || cols > HPCDNN_EXPERTS_MAX_COLS) return HPCDNN_ERR_INVALID_VALUE;
     if (tokens == 0 || cols == 0) return HPCDNN_OK;
     if ((rows > 0 && !rows_valid(xs, ldxs, cols, type)) || !rows_valid(y, ldy, cols, type) || pos == nullptr || !aligned(pos, 4) ||
         !aligned(weights, 4))
         return HPCDNN_ERR_INVALID_VALUE;
-    return with_type(type, [&](auto* t) {
+    const size_t e = type_bytes(type);
+    return with_rows(type, rows_are_dwords(xs, ldxs, cols, e) && rows_are_dwords(y, ldy, cols, e), [&](auto* t, auto dwords) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
         const dim3 grid(token_grid(tokens), static_cast<unsigned>(ceil_div(cols, kRowThreads * kVec<T>)));
-        if (grid.y > 65535) return HPCDNN_ERR_INVALID_VALUE;
-        expert_combine_kernel<T><<<grid, kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
+        expert_combine_kernel<T, decltype(dwords)::value><<<grid, kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
             tokens, topk, rows, cols, static_cast<const T*>(xs), ldxs, pos, weights, static_cast<T*>(y), ldy);
         return launch_status();
     });
@@ -318,15 +364,18 @@ extern "C" int hpcdnn_expert_combine_grad(int type, int tokens, int topk, int ro
                                           int64_t ldxs, const int32_t* pos, const float* weights, void* dxs, int64_t lddxs,
                                           float* dweights, void* stream) {
     using namespace hpcdnn;
-    if (!type_valid(type) || !choices_valid(tokens, topk) || rows < 0 || cols < 0) return HPCDNN_ERR_INVALID_VALUE;
+    if (!type_valid(type) || !choices_valid(tokens, topk) || rows < 0 || cols < 0 || cols > HPCDNN_EXPERTS_MAX_COLS) return HPCDNN_ERR_INVALID_VALUE;
     if (tokens == 0 || (dxs == nullptr && dweights == nullptr)) return HPCDNN_OK;
     if (pos == nullptr || !aligned(pos, 4) || !aligned(weights, 4) || !aligned(dweights, 4)) return HPCDNN_ERR_INVALID_VALUE;
     if (cols > 0 && (!rows_valid(dy, lddy, cols, type) || (rows > 0 && dweights && !rows_valid(xs, ldxs, cols, type)) ||
                      (rows > 0 && dxs && !rows_valid(dxs, lddxs, cols, type))))
         return HPCDNN_ERR_INVALID_VALUE;
-    return with_type(type, [&](auto* t) {
+    const size_t e = type_bytes(type);
+    const bool all_dwords = rows_are_dwords(dy, lddy, cols, e) && (dweights == nullptr || rows_are_dwords(xs, ldxs, cols, e)) &&
+                            (dxs == nullptr || rows_are_dwords(dxs, lddxs, cols, e));
+    return with_rows(type, all_dwords, [&](auto* t, auto dwords) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
-        expert_combine_grad_kernel<T><<<token_grid(tokens), kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
+        expert_combine_grad_kernel<T, decltype(dwords)::value><<<token_grid(tokens), kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
             tokens, topk, rows, cols, static_cast<const T*>(dy), lddy, static_cast<const T*>(xs), ldxs, pos, weights,
             static_cast<T*>(dxs), lddxs, dweights);
         return launch_status();

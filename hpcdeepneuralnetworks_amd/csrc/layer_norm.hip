@@ -14,36 +14,37 @@ namespace hpcdnn {
 constexpr int kNormRowWaves = 4;     // rows per workgroup where a wave takes a row of its own
 constexpr int kNormMaxWaves = 16;
 
-// Columns of the calling thread: vector v starts at column (v * team + lane_in_team) * kVec.
-template <class T, int NV>
-struct row_slice {
-    int col[NV];
-    __device__ row_slice(int t, int team) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) col[v] = (v * team + t) * kVec<T>;
-    }
-    __device__ void load(const T* row, int cols, v4u (&u)[NV]) const {
-#pragma unroll
-        for (int v = 0; v < NV; ++v) u[v] = load_row(row, col[v], cols);
-    }
-};
-
 // Parameters of the thread's columns in FP32; `fill` where there are none (and behind the last column).
-template <class T, class W, int NV>
-__device__ __forceinline__ void load_params(const W* p, float fill, const row_slice<T, NV>& s, int cols, float (&out)[NV][kVec<T>]) {
+template <class T, class W, int NV, bool kDwords>
+__device__ __forceinline__ void load_params(const W* p, float fill, const row_values<T, NV, kDwords>& s, int cols, float (&out)[NV][kVec<T>]) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
 #pragma unroll
-        for (int i = 0; i < kVec<T>; ++i)
-            out[v][i] = (p != nullptr && s.col[v] + i < cols) ? static_cast<float>(p[s.col[v] + i]) : fill;
+        for (int i = 0; i < kVec<T>; ++i) out[v][i] = fill;
+        if (p == nullptr) continue;
+        if constexpr (kDwords) {
+#pragma unroll
+            for (int i = 0; i < kVec<T>; i += kVec<W>) {
+                if (s.column(v, i) >= cols) continue;
+                float f[kVec<W>];
+                unpack<W>(load_row(p, s.column(v, i), cols), f);
+#pragma unroll
+                for (int k = 0; k < kVec<W>; ++k) out[v][i + k] = f[k];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i)
+                if (s.column(v, i) < cols) out[v][i] = static_cast<float>(p[s.column(v, i)]);
+        }
+    }
 }
 
 // One row per wave (kWaveRow: no exchange between waves) or per workgroup.  The mean and the squared deviations of a
 // wave's part of the row are formed in two passes over registers, the parts then joined exactly,
 //   mu = sum n_w mu_w / C,   M2 = sum M2_w + n_w (mu_w - mu)^2,
 // so nothing cancels (sum x^2 - C mu^2 would lose the variance of rows with a large mean) and a row costs one barrier.
-// The next row of the workgroup is loaded before the present one is reduced.
-template <class T, class W, int NV, bool kWaveRow>
+// The next row is loaded into the registers of the present one as soon as that is unpacked.
+template <class T, class W, int NV, bool kWaveRow, bool kDwords>
 __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer_norm_kernel(
     int64_t rows, int cols, const T* __restrict__ x, int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, float eps,
     T* __restrict__ y, int64_t ldy, float* __restrict__ mean, float* __restrict__ rstd) {
@@ -54,43 +55,42 @@ __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer
     const int64_t step = kWaveRow ? static_cast<int64_t>(gridDim.x) * kNormRowWaves : gridDim.x;
     int64_t r = kWaveRow ? static_cast<int64_t>(blockIdx.x) * kNormRowWaves + wave : blockIdx.x;
     if (r >= rows) return;
-    const row_slice<T, NV> s(kWaveRow ? lane : threadIdx.x, kWaveRow ? kWave : blockDim.x);
+    row_values<T, NV, kDwords> cur(kWaveRow ? lane : threadIdx.x, kWaveRow ? kWave : blockDim.x);
+    auto load = [&](int64_t row) { cur.load(x + (row < rows ? row : 0) * ldx, row < rows ? cols : 0); };
+    load(r);
+    float wf[NV][kVec<T>], bf[NV][kVec<T>];
+    load_params<T, W, NV, kDwords>(w, 1.f, cur, cols, wf);
+    load_params<T, W, NV, kDwords>(b, 0.f, cur, cols, bf);
     int valid = 0;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) valid += max(0, min(kVec<T>, cols - s.col[v]));
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < kVec<T>; ++i) valid += cur.column(v, i) < cols;
     const float n_wave = wave_allsum(static_cast<float>(valid));
     const float n_cols = static_cast<float>(cols);
     // columns of wave (lane & 15): what the join below weighs that wave's mean with
     float n_of_lane = 0.f;
     if (!kWaveRow) {
-        if (lane == 0) part[0][0][wave] = n_wave;
+        if (lane == 0) part[1][0][wave] = n_wave;
         __syncthreads();
-        n_of_lane = (lane & 15) < waves ? part[0][0][lane & 15] : 0.f;
-        __syncthreads();
+        n_of_lane = (lane & 15) < waves ? part[1][0][lane & 15] : 0.f;
     }
 
-    v4u cur[NV], nxt[NV];
-    s.load(x + r * ldx, cols, cur);
-    float wf[NV][kVec<T>], bf[NV][kVec<T>];
-    load_params<T, W, NV>(w, 1.f, s, cols, wf);
-    load_params<T, W, NV>(b, 0.f, s, cols, bf);
-    for (int turn = 0;; turn ^= 1) {
-        const int64_t next = r + step;
-        if (next < rows) s.load(x + next * ldx, cols, nxt);
+    for (int turn = 0; r < rows; r += step, turn ^= 1) {
         float f[NV][kVec<T>], sum = 0.f;
+        cur.get(f);
+        load(r + step);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            unpack<T>(cur[v], f[v]);
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) sum += f[v][i];
-        }
         // divided, not multiplied by a reciprocal: a row of equal values then has exactly that mean, and no spread
         float mu = wave_allsum(sum) / fmaxf(n_wave, 1.f), m2 = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) {
-                const float d = s.col[v] + i < cols ? f[v][i] - mu : 0.f;
+                const float d = cur.column(v, i) < cols ? f[v][i] - mu : 0.f;
                 m2 = __builtin_fmaf(d, d, m2);
             }
         m2 = wave_allsum(m2);
@@ -107,63 +107,71 @@ __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer
         }
         const float rs = 1.f / __builtin_sqrtf(m2 / n_cols + eps);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            float o[kVec<T>];
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int i = 0; i < kVec<T>; ++i) o[i] = __builtin_fmaf((f[v][i] - mu) * rs, wf[v][i], bf[v][i]);
-            store_row(y + r * ldy, s.col[v], cols, pack<T>(o));
-        }
+            for (int i = 0; i < kVec<T>; ++i) f[v][i] = __builtin_fmaf((f[v][i] - mu) * rs, wf[v][i], bf[v][i]);
+        cur.store(y + r * ldy, cols, f);
         if ((kWaveRow ? lane : static_cast<int>(threadIdx.x)) == 0) {
             if (mean != nullptr) mean[r] = mu;
             if (rstd != nullptr) rstd[r] = rs;
         }
-        if (next >= rows) break;
-        r = next;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) cur[v] = nxt[v];
     }
 }
 
-// Gradient.  A workgroup walks its rows (workgroup, workgroup + grid, ...), adding dy xh and dy of its columns in
-// registers, and writes one partial row of each at the end: [workgroup][2][cols] in the workspace, added in the
-// workgroups' order by layer_norm_params_kernel, so dw and db do not depend on timing.
-template <class T, class W, int NV, bool kWaveRow>
-__global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer_norm_grad_kernel(
-    int64_t rows, int cols, const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx, const W* __restrict__ w,
-    const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx, int64_t lddx, float* __restrict__ partial) {
+// Gradient.  A workgroup is several teams of `row_waves` waves, each with a row at a time: rows (workgroup, team), then
+// every grid * teams further.  A thread adds dy xh and dy of its columns in registers; the teams' sums are joined in LDS in
+// their order at the end, and the workgroup writes one partial row of each, [workgroup][2][cols] in the workspace, added in
+// the workgroups' order by layer_norm_params_kernel.  So dw and db do not depend on timing, and with sixteen waves to a
+// workgroup the partial rows stay few: they are the only traffic beside x, dy and dx.
+template <class T, class W, int NV, bool kWaveRow, bool kDwords>
+__global__ __launch_bounds__(1024) void layer_norm_grad_kernel(
+    int64_t rows, int cols, int row_waves, const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
+    const W* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx, int64_t lddx,
+    float* __restrict__ partial) {
     __shared__ float part[2][2][kNormMaxWaves];
-    extern __shared__ float joined[];  // kWaveRow: [2][cols], the waves' sums added in wave order
+    extern __shared__ float joined[];  // [2][values of a thread][pitch] where there are several teams
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int waves = blockDim.x / kWave;
-    const int64_t step = kWaveRow ? static_cast<int64_t>(gridDim.x) * kNormRowWaves : gridDim.x;
-    int64_t r = kWaveRow ? static_cast<int64_t>(blockIdx.x) * kNormRowWaves + wave : blockIdx.x;
-    const row_slice<T, NV> s(kWaveRow ? lane : threadIdx.x, kWaveRow ? kWave : blockDim.x);
+    if (kWaveRow) row_waves = 1;
+    const int teams = (blockDim.x / kWave) / row_waves, team = kWaveRow ? wave : __builtin_amdgcn_readfirstlane(wave / row_waves);
+    const int first_wave = team * row_waves;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
+    const int64_t block_row = static_cast<int64_t>(blockIdx.x) * teams;
+    int64_t r = block_row + team;
+    row_values<T, NV, kDwords> cx((wave - first_wave) * kWave + lane, row_waves * kWave), cd(cx.t, cx.n);
     const float inv_cols = 1.f / static_cast<float>(cols);
+    constexpr bool kKeep = NV * kVec<T> <= 8;  // w in registers; wider rows read it again (from L2), or they would spill
     float wf[NV][kVec<T>], dw[NV][kVec<T>], db[NV][kVec<T>];
-    load_params<T, W, NV>(w, 1.f, s, cols, wf);
+    if (kKeep) load_params<T, W, NV, kDwords>(w, 1.f, cx, cols, wf);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int i = 0; i < kVec<T>; ++i) dw[v][i] = db[v][i] = 0.f;
-    v4u cx[NV], cd[NV], nx[NV], nd[NV];
-    if (r < rows) {
-        s.load(x + r * ldx, cols, cx);
-        s.load(dy + r * lddy, cols, cd);
-    }
-    for (int turn = 0; r < rows; turn ^= 1) {
-        const int64_t next = r + step;
-        if (next < rows) {
-            s.load(x + next * ldx, cols, nx);
-            s.load(dy + next * lddy, cols, nd);
-        }
-        const float mu = mean[r], rs = rstd[r];
+    float next_mu, next_rs;
+    // Behind the last row: zeros, which add nothing.  The statistics come as vector loads too: a scalar load in flight
+    // would be waited for with the LDS accesses of the exchange between the waves, which share its counter.
+    auto load = [&](int64_t row) {
+        const bool is = row < rows;
+        const int64_t at = is ? row : 0;
+        cx.load(x + at * ldx, is ? cols : 0);
+        cd.load(dy + at * lddy, is ? cols : 0);
+        next_mu = buffer_load_f(make_rsrc(mean + at, is ? 4 : 0), 0);
+        next_rs = buffer_load_f(make_rsrc(rstd + at, is ? 4 : 0), 0);
+    };
+    load(r);
+    int turn = 0;
+    // all teams walk as long as the first has rows: the barrier is the workgroup's
+    for (int64_t lead = block_row; lead < rows; lead += step, r += step, turn ^= 1) {
+        // into scalar registers, so that the next row's can be on their way in these
+        const float mu = wave_first(next_mu), rs = wave_first(next_rs);
         float g_sum = 0.f, gx_sum = 0.f;
         float xh[NV][kVec<T>], g[NV][kVec<T>];
+        cx.get(xh);
+        cd.get(g);
+        if (!kKeep) load_params<T, W, NV, kDwords>(w, 1.f, cx, cols, wf);
+        load(r + step);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            unpack<T>(cx[v], xh[v]);
-            unpack<T>(cd[v], g[v]);
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) {
                 xh[v][i] = (xh[v][i] - mu) * rs;
@@ -173,81 +181,84 @@ __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer
                 g_sum += g[v][i];
                 gx_sum = __builtin_fmaf(g[v][i], xh[v][i], gx_sum);
             }
-        }
-        if (dx != nullptr) {
-            g_sum = wave_allsum(g_sum);
-            gx_sum = wave_allsum(gx_sum);
-            if (!kWaveRow) {
-                if (lane == 0) {
-                    part[turn][0][wave] = g_sum;
-                    part[turn][1][wave] = gx_sum;
-                }
-                __syncthreads();
-                const bool has = (lane & 15) < waves;
-                g_sum = row16_allsum(has ? part[turn][0][lane & 15] : 0.f);
-                gx_sum = row16_allsum(has ? part[turn][1][lane & 15] : 0.f);
+        g_sum = wave_allsum(g_sum);
+        gx_sum = wave_allsum(gx_sum);
+        if (!kWaveRow) {
+            if (lane == 0) {
+                part[turn][0][wave] = g_sum;
+                part[turn][1][wave] = gx_sum;
             }
-            const float a = g_sum * inv_cols, c = gx_sum * inv_cols;
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                float o[kVec<T>];
-#pragma unroll
-                for (int i = 0; i < kVec<T>; ++i) o[i] = rs * (g[v][i] - a - xh[v][i] * c);
-                store_row(dx + r * lddx, s.col[v], cols, pack<T>(o));
-            }
+            __syncthreads();
+            const bool has = (lane & 15) < row_waves;
+            g_sum = row16_allsum(has ? part[turn][0][first_wave + (lane & 15)] : 0.f);
+            gx_sum = row16_allsum(has ? part[turn][1][first_wave + (lane & 15)] : 0.f);
         }
-        r = next;
+        const float a = g_sum * inv_cols, c = gx_sum * inv_cols;
+        const bool is = r < rows && dx != nullptr;  // else dropped
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            cx[v] = nx[v];
-            cd[v] = nd[v];
-        }
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i) g[v][i] = rs * (g[v][i] - a - xh[v][i] * c);
+        cx.store(dx + (is ? r : 0) * lddx, is ? cols : 0, g);
     }
     if (partial == nullptr) return;
     float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * cols;
-    if (kWaveRow) {
-        for (int turn = 0; turn < kNormRowWaves; ++turn) {
-            if (turn == wave) {
-#pragma unroll
-                for (int v = 0; v < NV; ++v)
-#pragma unroll
-                    for (int i = 0; i < kVec<T>; ++i) {
-                        const int c = s.col[v] + i;
-                        if (c < cols) {
-                            joined[c] = turn == 0 ? dw[v][i] : joined[c] + dw[v][i];
-                            joined[cols + c] = turn == 0 ? db[v][i] : joined[cols + c] + db[v][i];
-                        }
-                    }
-            }
-            __syncthreads();
-        }
-        for (int i = threadIdx.x; i < 2 * cols; i += blockDim.x) out[i] = joined[i];
-    } else {
+    if (teams == 1) {
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) {
-                const int c = s.col[v] + i;
+                const int c = cx.column(v, i);
                 if (c < cols) {
                     out[c] = dw[v][i];
                     out[cols + c] = db[v][i];
                 }
             }
+        return;
+    }
+    // value i of thread t of a team at i * pitch + t, dw and db in turn: neither the threads nor, with a pitch of 8 mod 64,
+    // the walk over the columns below meet a bank twice
+    const int n = cx.n, pitch = n + 8;
+    for (int k = 0; k < teams; ++k) {
+        if (k == team) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int i = 0; i < kVec<T>; ++i) {
+                    float* a = joined + (v * kVec<T> + i) * pitch + cx.t;
+                    float* b = a + NV * kVec<T> * pitch;
+                    *a = k == 0 ? dw[v][i] : *a + dw[v][i];
+                    *b = k == 0 ? db[v][i] : *b + db[v][i];
+                }
+        }
+        __syncthreads();
+    }
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+        int value = c / n, thread = c - value * n;
+        if (kDwords) {
+            const int vec = c / kVec<T>, v = vec / n;
+            value = v * kVec<T> + c % kVec<T>;
+            thread = vec - v * n;
+        }
+        const float* a = joined + value * pitch + thread;
+        out[c] = a[0];
+        out[cols + c] = a[NV * kVec<T> * pitch];
     }
 }
 
-// dw[c], db[c] = the partial rows added in order: 32 columns by 8 runs of consecutive partial rows per workgroup, the
-// runs added in order.
+// dw[c], db[c] = the partial rows added in order: 32 columns by 32 runs of consecutive partial rows per workgroup, the
+// runs added in order.  Few enough columns for a handful of workgroups, so the rows are what is spread over the threads.
+constexpr int kParamsRuns = 32;
 template <class W>
-__global__ __launch_bounds__(256) void layer_norm_params_kernel(int parts, int cols, const float* __restrict__ partial, W* __restrict__ dw,
-                                                                W* __restrict__ db) {
-    __shared__ float run[8][32];
+__global__ __launch_bounds__(32 * kParamsRuns) void layer_norm_params_kernel(int parts, int cols, const float* __restrict__ partial,
+                                                                             W* __restrict__ dw, W* __restrict__ db) {
+    __shared__ float run[kParamsRuns][32];
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x / 32;
-    const int per = (parts + 7) / 8;
+    const int per = (parts + kParamsRuns - 1) / kParamsRuns;
     const int first = k * per, last = min(parts, first + per);
     float sum = 0.f;
     if (c < 2 * cols) {
-        constexpr int kBatch = 8;
+        constexpr int kBatch = 16;
         for (int p = first; p < last; p += kBatch) {
             float t[kBatch];
 #pragma unroll
@@ -260,7 +271,7 @@ __global__ __launch_bounds__(256) void layer_norm_params_kernel(int parts, int c
     __syncthreads();
     if (k != 0 || c >= 2 * cols) return;
 #pragma unroll
-    for (int u = 1; u < 8; ++u) sum += run[u][threadIdx.x];
+    for (int u = 1; u < kParamsRuns; ++u) sum += run[u][threadIdx.x];
     if (c < cols) {
         if (dw != nullptr) dw[c] = static_cast<W>(sum);
     } else if (db != nullptr) {
@@ -283,12 +294,25 @@ norm_shape shape_of(int cols, int vec) {
     return {false, nv, static_cast<int>(ceil_div(ceil_div(vecs, nv), kWave)) * kWave};
 }
 
-// Most workgroups of the gradient, each of which leaves a partial row of dw and db: a function of the sizes and the CU
-// count alone, so the workspace does not depend on the type.
-int grad_blocks(int rows, int cols) {
-    const int per_cu = cols <= 2048 ? 4 : cols <= 4096 ? 2 : 1;
-    const int most = device_cus() * per_cu;
-    return rows < most ? rows : most;
+// Most workgroups of the gradient, each of which leaves a partial row of dw and db: one per CU, whatever the type.  (Two per
+// CU measured 2 % faster for 30000 x 512 BF16, but 5 to 11 % slower from 2048 columns on: the partial rows double.)
+int grad_blocks(int rows) { return std::min(rows, device_cus()); }
+
+// f(NV, kWaveRow, kDwords) as compile-time constants
+template <class T, class F>
+void with_shape(const norm_shape& s, bool dwords, F&& f) {
+    using std::integral_constant;
+    auto more = [&](auto nv, auto wave_row) {
+        if constexpr (sizeof(T) == 4) f(nv, wave_row, std::true_type{});
+        else if (dwords) f(nv, wave_row, std::true_type{});
+        else f(nv, wave_row, std::false_type{});
+    };
+    if (s.wave_row) {
+        if (s.nv == 1) more(integral_constant<int, 1>{}, std::true_type{});
+        else more(integral_constant<int, 2>{}, std::true_type{});
+    } else if (s.nv == 1) more(integral_constant<int, 1>{}, std::false_type{});
+    else if (s.nv == 2) more(integral_constant<int, 2>{}, std::false_type{});
+    else if constexpr (kVec<T> == 4) more(integral_constant<int, 4>{}, std::false_type{});
 }
 
 template <class T, class W>
@@ -298,18 +322,11 @@ int launch_norm(int rows, int cols, const void* x, int64_t ldx, const void* w, c
     const int64_t blocks = s.wave_row ? ceil_div(rows, kNormRowWaves) : rows;
     const int64_t most = static_cast<int64_t>(device_cus()) * (2048 / s.threads);
     const int grid = static_cast<int>(blocks < most ? blocks : most);
-    auto go = [&](auto nv, auto wave_row) {
-        layer_norm_kernel<T, W, decltype(nv)::value, decltype(wave_row)::value><<<grid, s.threads, 0, stream>>>(
+    with_shape<T>(s, rows_are_dwords(x, ldx, cols, sizeof(T)) && rows_are_dwords(y, ldy, cols, sizeof(T)), [&](auto nv, auto wave_row, auto dwords) {
+        layer_norm_kernel<T, W, decltype(nv)::value, decltype(wave_row)::value, decltype(dwords)::value><<<grid, s.threads, 0, stream>>>(
             rows, cols, static_cast<const T*>(x), ldx, static_cast<const W*>(w), static_cast<const W*>(b), eps, static_cast<T*>(y), ldy,
             mean, rstd);
-    };
-    using std::integral_constant;
-    if (s.wave_row) {
-        if (s.nv == 1) go(integral_constant<int, 1>{}, std::true_type{});
-        else go(integral_constant<int, 2>{}, std::true_type{});
-    } else if (s.nv == 1) go(integral_constant<int, 1>{}, std::false_type{});
-    else if (s.nv == 2) go(integral_constant<int, 2>{}, std::false_type{});
-    else if constexpr (kVec<T> == 4) go(integral_constant<int, 4>{}, std::false_type{});
+    });
     return launch_status();
 }
 
@@ -317,26 +334,23 @@ template <class T, class W>
 int launch_grad(int rows, int cols, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const float* mean,
                 const float* rstd, void* dx, int64_t lddx, void* dw, void* db, float* partial, hipStream_t stream) {
     const norm_shape s = shape_of(cols, kVec<T>);
-    int grid = grad_blocks(rows, cols);
-    if (s.wave_row) grid = std::min(grid, static_cast<int>(ceil_div(rows, kNormRowWaves)));
+    const int row_waves = s.wave_row ? 1 : s.threads / kWave;
+    const int teams = s.wave_row ? 8 : kNormMaxWaves / row_waves;
+    const int grid = std::min(grad_blocks(rows), static_cast<int>(ceil_div(rows, teams)));
     if (grid > 0) {
-        const size_t lds = s.wave_row && partial ? 2 * static_cast<size_t>(cols) * sizeof(float) : 0;
-        auto go = [&](auto nv, auto wave_row) {
-            layer_norm_grad_kernel<T, W, decltype(nv)::value, decltype(wave_row)::value><<<grid, s.threads, lds, stream>>>(
-                rows, cols, static_cast<const T*>(dy), lddy, static_cast<const T*>(x), ldx, static_cast<const W*>(w), mean, rstd,
-                static_cast<T*>(dx), lddx, partial);
-        };
-        using std::integral_constant;
-        if (s.wave_row) {
-            if (s.nv == 1) go(integral_constant<int, 1>{}, std::true_type{});
-            else go(integral_constant<int, 2>{}, std::true_type{});
-        } else if (s.nv == 1) go(integral_constant<int, 1>{}, std::false_type{});
-        else if (s.nv == 2) go(integral_constant<int, 2>{}, std::false_type{});
-        else if constexpr (kVec<T> == 4) go(integral_constant<int, 4>{}, std::false_type{});
+        const size_t lds = teams > 1 && partial ? 2 * sizeof(float) * s.nv * kVec<T> * (row_waves * kWave + 8) : 0;
+        const bool all_dwords = rows_are_dwords(x, ldx, cols, sizeof(T)) && rows_are_dwords(dy, lddy, cols, sizeof(T)) &&
+                                (dx == nullptr || rows_are_dwords(dx, lddx, cols, sizeof(T)));
+        with_shape<T>(s, all_dwords, [&](auto nv, auto wave_row, auto dwords) {
+            layer_norm_grad_kernel<T, W, decltype(nv)::value, decltype(wave_row)::value, decltype(dwords)::value>
+                <<<grid, teams * row_waves * kWave, lds, stream>>>(
+                    rows, cols, row_waves, static_cast<const T*>(dy), lddy, static_cast<const T*>(x), ldx, static_cast<const W*>(w), mean,
+                    rstd, static_cast<T*>(dx), lddx, partial);
+        });
         if (int e = launch_status()) return e;
     }
     if (partial != nullptr || (grid == 0 && (dw || db)))
-        layer_norm_params_kernel<W><<<static_cast<int>(ceil_div(2 * static_cast<int64_t>(cols), 32)), 256, 0, stream>>>(
+        layer_norm_params_kernel<W><<<static_cast<int>(ceil_div(2 * static_cast<int64_t>(cols), 32)), 32 * kParamsRuns, 0, stream>>>(
             grid, cols, partial, static_cast<W*>(dw), static_cast<W*>(db));
     return launch_status();
 }
@@ -362,7 +376,7 @@ int with_types(int type, int wtype, F&& f) {
 
 size_t layer_norm_grad_workspace_bytes(int rows, int cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    return static_cast<size_t>(grad_blocks(rows, cols)) * 2 * cols * sizeof(float);
+    return static_cast<size_t>(grad_blocks(rows)) * 2 * cols * sizeof(float);
 }
 
 }  // namespace hpcdnn

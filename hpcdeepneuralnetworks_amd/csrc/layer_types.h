@@ -23,9 +23,9 @@ template <class T>
 __device__ __forceinline__ v4u load16(const T* p) {
     return *reinterpret_cast<const v4u_any*>(p);
 }
-template <class T>
-__device__ __forceinline__ void store16(T* p, v4u v) {
-    *reinterpret_cast<v4u_any*>(p) = v;
+// One float through a descriptor.
+__device__ __forceinline__ float buffer_load_f(__amdgpu_buffer_rsrc_t rs, int byte_offset) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rs, byte_offset, 0, 0));
 }
 
 // The first `n` values of such a vector, 0 < n < kVec<T>; zeros behind them.
@@ -60,10 +60,10 @@ __device__ __forceinline__ v4u load_row(const T* row, int col, int cols) {
     if (col < cols) return load_part(row + col, cols - col);
     return v4u{0u, 0u, 0u, 0u};
 }
-template <class T>
-__device__ __forceinline__ void store_row(T* row, int col, int cols, v4u v) {
-    if (col + kVec<T> <= cols) store16(row + col, v);
-    else if (col < cols) store_part(row + col, v, cols - col);
+
+// Whether rows of this matrix are whole dwords (host).
+inline bool rows_are_dwords(const void* p, int64_t ld, int cols, size_t elem) {
+    return reinterpret_cast<uintptr_t>(p) % 4 == 0 && (ld * static_cast<int64_t>(elem)) % 4 == 0 && (cols * elem) % 4 == 0;
 }
 
 template <class T>
@@ -106,9 +106,95 @@ __device__ __forceinline__ v4u pack(const float (&f)[kVec<T>]) {
     return u;
 }
 
+// A row of `cols` values (0: no row at all) as a buffer descriptor, wave-uniform.  Loads give zeros behind the end and
+// stores there are dropped, without a branch.  That is worth more than the instructions it saves: loads and stores share one
+// in-order counter, and behind a store in a branch the wait for an older load has to be one for every store as well.
+// 16 bytes at a time need a row on a 4-byte address that holds whole dwords (the range check is per dword).
+template <class T, bool kDwords>
+struct row_buffer {
+    __amdgpu_buffer_rsrc_t rs;
+    int skew;  // bytes by which the row starts behind a 4-byte address (rows that are read by single values)
+    __device__ __forceinline__ row_buffer(const T* row, int cols) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(row);
+        skew = kDwords ? 0 : static_cast<int>(at & 2);
+        const int64_t bytes = static_cast<int64_t>(cols) * static_cast<int64_t>(sizeof(T));
+        rs = make_rsrc(reinterpret_cast<const float*>(at - skew), kDwords ? bytes : cols > 0 ? bytes + skew : 0);
+    }
+    __device__ __forceinline__ v4u load16(int col) const {
+        return __builtin_amdgcn_raw_buffer_load_b128(rs, col * static_cast<int>(sizeof(T)), 0, 0);
+    }
+    // non-temporal: a large result that nothing on the way reads again
+    __device__ __forceinline__ void store16_once(int col, v4u v) const {
+        __builtin_amdgcn_raw_buffer_store_b128(v, rs, col * static_cast<int>(sizeof(T)), 0, 2);
+    }
+    __device__ __forceinline__ T load1(int col) const {
+        return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(rs, col * 2 + skew, 0, 0));
+    }
+    __device__ __forceinline__ void store1(int col, T v) const {
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), rs, col * 2 + skew, 0, 0);
+    }
+};
+
+// The values of a row that one thread of the `n` that share it holds, NV vectors of kVec.  kDwords: consecutive values, 16
+// bytes at a time, vector v from column (v n + t) kVec on.  Else (16-bit rows that start at odd addresses or hold an odd
+// number of values) single ones, n apart, so that the threads of a wave still touch consecutive addresses.
+template <class T, int NV, bool kDwords>
+struct row_values {
+    static_assert(kDwords || sizeof(T) == 2, "FP32 rows are whole dwords");
+    int t, n;
+    v4u u[kDwords ? NV : 1];
+    T single[kDwords ? 1 : NV * kVec<T>];
+    __device__ __forceinline__ row_values(int thread, int threads) : t(thread), n(threads) {}
+    __device__ __forceinline__ int column(int v, int i) const { return kDwords ? (v * n + t) * kVec<T> + i : (v * kVec<T> + i) * n + t; }
+    __device__ __forceinline__ void load(const T* row, int cols) {
+        const row_buffer<T, kDwords> b(row, cols);
+        if constexpr (kDwords) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) u[v] = b.load16(column(v, 0));
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV * kVec<T>; ++k) single[k] = b.load1(k * n + t);
+        }
+    }
+    __device__ __forceinline__ void get(float (&f)[NV][kVec<T>]) const {
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if constexpr (kDwords) unpack<T>(u[v], f[v]);
+            else
+#pragma unroll
+                for (int i = 0; i < kVec<T>; ++i) f[v][i] = static_cast<float>(single[v * kVec<T> + i]);
+        }
+    }
+    __device__ __forceinline__ void copy_to(T* row, int cols) const {
+        const row_buffer<T, kDwords> b(row, cols);
+        if constexpr (kDwords) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) b.store16_once(column(v, 0), u[v]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < NV * kVec<T>; ++k) b.store1(k * n + t, single[k]);
+        }
+    }
+    __device__ __forceinline__ void store(T* row, int cols, const float (&f)[NV][kVec<T>]) const {
+        const row_buffer<T, kDwords> b(row, cols);
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            if constexpr (kDwords) b.store16_once(column(v, 0), pack<T>(f[v]));
+            else
+#pragma unroll
+                for (int i = 0; i < kVec<T>; ++i) b.store1(column(v, i), static_cast<T>(f[v][i]));
+        }
+    }
+};
+
 // Sum over the wave, in every lane (a scalar register: the value is read from lane 63).
 __device__ __forceinline__ float wave_allsum(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_sum_lane63(v)), 63));
+}
+
+// The value of the first lane, for one that is the same in all: a scalar register.
+__device__ __forceinline__ float wave_first(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
 }
 
 inline size_t type_bytes(int type) { return type == HPCDNN_F32 ? 4 : 2; }

@@ -510,9 +510,11 @@ int hpcdnn_w4_quantize(int type, int M, int N, int group, const float* W, int64_
  *   offsets[e]   first place of expert e, e = 0 .. experts
  * (pos is tokens x topk without gaps.)  `ws`: hpcdnn_workspace_bytes(HPCDNN_OP_EXPERT_SORT, tokens, topk,
  * experts) bytes (0 for few tokens), 16-byte aligned, no initialisation.
- * experts <= HPCDNN_EXPERTS_MAX, topk <= HPCDNN_EXPERTS_MAX_TOPK, tokens * topk < 2^31. */
+ * experts <= HPCDNN_EXPERTS_MAX, topk <= HPCDNN_EXPERTS_MAX_TOPK, tokens * topk < 2^31; rows hold at most
+ * HPCDNN_EXPERTS_MAX_COLS columns (below). */
 #define HPCDNN_EXPERTS_MAX 512
 #define HPCDNN_EXPERTS_MAX_TOPK 64
+#define HPCDNN_EXPERTS_MAX_COLS (1 << 24)
 int hpcdnn_expert_sort(int tokens, int topk, int experts, const int32_t* ids, int64_t ldids, int32_t* offsets, int32_t* pos,
                        int32_t* order, void* ws, size_t ws_bytes, void* stream);
 /* out[pos[t][j]] = x[t]: the rows of x (tokens x cols) at the places of their choices.  A place outside 0 .. rows-1 is
