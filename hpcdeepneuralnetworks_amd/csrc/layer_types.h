@@ -187,6 +187,10 @@ struct row_values {
     }
 };
 
+// Put behind loads whose values are for the next turn of a loop: memory might have changed, as far as the compiler knows, so
+// it cannot move them (as it does with plain loads) to where that turn uses them, and they stay in flight over this one.
+__device__ __forceinline__ void loads_start_here() { asm volatile("" ::: "memory"); }
+
 // Sum over the wave, in every lane (a scalar register: the value is read from lane 63).
 __device__ __forceinline__ float wave_allsum(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wave_sum_lane63(v)), 63));

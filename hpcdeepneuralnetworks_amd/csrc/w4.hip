@@ -14,21 +14,6 @@
 #include <cmath>
 
 #include "layer_types.h"
-#ifndef W4MIN
-#define W4MIN 5
-#endif
-#ifndef W4TW
-#define W4TW kW4TileWaves
-#endif
-#ifndef W4BPC
-#define W4BPC 1
-#endif
-#ifndef W4ROWS
-#define W4ROWS
-#endif
-#ifndef W4RT
-#define W4RT 1
-#endif
 
 namespace hpcdnn {
 
@@ -46,17 +31,20 @@ __device__ __forceinline__ v4u pair_order(v4u d) {
                __builtin_amdgcn_perm(d[3], d[1], 0x05040100u), __builtin_amdgcn_perm(d[3], d[1], 0x07060302u)};
 }
 
-// The eight nibbles of w as 16 + q in T, columns (p, p + 4) in dword p.
+// The eight nibbles of w as 16 + q in T, columns (p, p + 4) in dword p: a shift and one v_bfi_b32 each.  An instruction takes
+// one constant from a scalar register and none from the instruction stream beside it, so the second has to be a vector
+// register; left to itself the compiler uses two instructions with a literal each instead.
 template <class T>
-__device__ __forceinline__ v4u nibbles_plus_16(unsigned w) {
-    if constexpr (std::is_same_v<T, f16>) {      // 16.0 = 0x4C00, q in bits 6 .. 9 of the mantissa
-        constexpr unsigned mask = 0x03C003C0u, one = 0x4C004C00u;
-        return v4u{((w << 6) & mask) | one, ((w << 2) & mask) | one, ((w >> 2) & mask) | one, ((w >> 6) & mask) | one};
-    } else {                                     // 16.0 = 0x4180, q in bits 3 .. 6
-        constexpr unsigned mask = 0x00780078u, one = 0x41804180u;
-        return v4u{((w << 3) & mask) | one, ((w >> 1) & mask) | one, ((w >> 5) & mask) | one, ((w >> 9) & mask) | one};
+struct nibble_maker {
+    static constexpr unsigned kMask = std::is_same_v<T, f16> ? 0x03C003C0u : 0x00780078u;  // where q stands in the mantissa of 16.0
+    unsigned one = std::is_same_v<T, f16> ? 0x4C004C00u : 0x41804180u;
+    __device__ __forceinline__ nibble_maker() { asm("" : "+v"(one)); }
+    __device__ __forceinline__ unsigned put(unsigned w) const { return (w & kMask) | (one & ~kMask); }
+    __device__ __forceinline__ v4u operator()(unsigned w) const {
+        if constexpr (std::is_same_v<T, f16>) return v4u{put(w << 6), put(w << 2), put(w >> 2), put(w >> 6)};
+        else return v4u{put(w << 3), put(w >> 1), put(w >> 5), put(w >> 9)};
     }
-}
+};
 
 template <class T>
 __device__ __forceinline__ float dot2(unsigned a, unsigned b, float c) {
@@ -110,6 +98,8 @@ __global__ __launch_bounds__(kW4MaxWaves * kWave) void w4_gemv_kernel(int batch,
     const int row_bytes = ((N + 1) / 2 + 3) & ~3;  // whole dwords: the last may hold bytes behind the row, whose x is zero
     const int first = blockIdx.x * rows_per_block, last = min(M, first + rows_per_block);
 
+    [[maybe_unused]] const nibble_maker<std::conditional_t<sizeof(T) == 2, T, f16>> nibbles;
+
     // rows r0 ... of the workgroup, columns from n0 + p0 * 2048 on
     v4u w[kRows][kPieces];
     T s[kRows][kPieces];
@@ -130,6 +120,7 @@ __global__ __launch_bounds__(kW4MaxWaves * kWave) void w4_gemv_kernel(int batch,
                 if (kZeros) z[r][u] = zeros[g];
             }
         }
+        loads_start_here();
     };
     if (first < last && N > 0) load(first, 0, 0);
     bool staged = false;
@@ -177,7 +168,7 @@ __global__ __launch_bounds__(kW4MaxWaves * kWave) void w4_gemv_kernel(int batch,
                                 xv[t] = *reinterpret_cast<const v4u*>(lds + (((t * pieces + p0 + u) * kW4Parts<T> + d) * kWave + lane) * 16);
 #pragma unroll
                             for (int r = 0; r < kRows; ++r) {
-                                const v4u wq = nibbles_plus_16<T>(now[r][u][d]);
+                                const v4u wq = nibbles(now[r][u][d]);
 #pragma unroll
                                 for (int t = 0; t < TB; ++t)
 #pragma unroll
@@ -232,12 +223,19 @@ __global__ __launch_bounds__(kW4MaxWaves * kWave) void w4_gemv_kernel(int batch,
 // rows by kTokTiles of tokens; its waves split the columns between them, in runs of units of 128, and their sums meet in
 // LDS at the end (in wave order): so a narrow matrix still keeps every CU loading.
 //
-// Lane l reads 16 bytes (32 columns) of row l % 16 from quarter l / 16 of the unit.  An instruction sums over the four
-// quarters of the lanes, so the dwords are first exchanged between the quarters (a 4 x 4 transposition in four lane swaps):
-// dword d of the lanes is then columns 32 d + 8 (l / 16) ... of the unit, and every instruction stays inside one group.
-// The sums over x that take out the offset of the nibbles come from the same instruction with a matrix of ones.
+// What limits it is the number of cache lines and 64-byte pieces that the loads touch: neighbouring lanes therefore load
+// neighbouring 16 bytes (four lanes a row's unit of weights, sixteen lanes a token's unit of x), and the order that the
+// instructions want, row or token l % 16 and part l / 16 in lane l, comes about in LDS, each wave for itself.  (Loaded in that
+// order right away, thirteen tokens by 6143 x 8200 took 20 us; scales go through LDS as well, sixteen of a row at a time.)
+//
+// An instruction sums over the four quarters of the lanes, so the dwords of the weights are exchanged between the quarters (a
+// 4 x 4 transposition in four lane swaps): dword d is then columns 32 d + 8 (l / 16) ... of the unit, and every instruction
+// stays inside one group.  The sums over x that take out the offset of the nibbles come from the same instruction with a
+// matrix of ones.
 constexpr int kW4Unit = 128;
-constexpr int kW4TileWaves = 16;
+constexpr int kW4TileTokens = 3;  // tokens from which this form is taken
+constexpr int kW4TileWaves = 8;
+constexpr int kW4Segment = 16;  // scales of a row that a wave keeps in LDS at a time
 
 typedef f16 v8h __attribute__((ext_vector_type(8)));
 typedef bf16 v8b __attribute__((ext_vector_type(8)));
@@ -258,13 +256,19 @@ __device__ __forceinline__ v4u transpose_quarters(v4u w) {
     return v4u{c[0], c[1], d[0], d[1]};
 }
 
+// LDS of a wave of the kernel below: its parts, or its sums at the end.
+constexpr int w4_tile_lds(int row_tiles, int tok_tiles) {
+    const int parts = 1024 + row_tiles * 16 * kW4Segment * 3, sums = row_tiles * tok_tiles * 4 * kWave * 4;
+    return parts > sums ? parts : sums;
+}
+
 template <class T, int kRowTiles, int kTokTiles, int kGroupSteps, bool kZeros>
-__global__ __launch_bounds__(W4TW * kWave) void w4_tile_kernel(int batch, int M, int N, float alpha,
+__global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch, int M, int N, float alpha,
                                                                        const unsigned char* __restrict__ q, int64_t ldq,
                                                                        const T* __restrict__ scales, const unsigned char* __restrict__ zeros,
                                                                        int64_t ldg, const T* __restrict__ x, int64_t ldx, float beta,
                                                                        T* __restrict__ y, int64_t ldy, int units_per_wave) {
-    extern __shared__ __align__(16) float part[];  // [wave][tile][4][lane]
+    extern __shared__ __align__(16) float part[];  // x of a unit per wave, at the end sums [wave][tile][4][lane]
     constexpr int kGroup = 32 * kGroupSteps, kGroups = 4 / kGroupSteps;  // columns of a group, groups of a unit
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int waves = blockDim.x / kWave;
@@ -272,19 +276,26 @@ __global__ __launch_bounds__(W4TW * kWave) void w4_tile_kernel(int batch, int M,
     const int m0 = blockIdx.x * kRowTiles * 16, t0 = blockIdx.y * kTokTiles * 16;
     const int full = N / kW4Unit, units = (N + kW4Unit - 1) / kW4Unit, groups = (N + kGroup - 1) / kGroup;
     const int begin = wave * units_per_wave, end = min(full & ~1, begin + units_per_wave);  // units_per_wave is even
+    // rows of the lane as the instructions want them (row) and as they are loaded (lane / 4)
+    auto row_at = [&](int tile, int i) { return static_cast<int64_t>(min(m0 + tile * 16 + i, M - 1)); };
     const unsigned char* wp[kRowTiles];
     const T* sp[kRowTiles];
     const unsigned char* zp[kRowTiles];
     const T* xp[kTokTiles];
+    const int load_row_of = lane >> 2, load_part = lane & 3;
 #pragma unroll
     for (int r = 0; r < kRowTiles; ++r) {
-        const int64_t m = min(m0 + r * 16 + row, M - 1);
-        wp[r] = q + m * ldq + quarter * 16;
+        const int64_t m = row_at(r, load_row_of);
+        wp[r] = q + m * ldq + load_part * 16;
         sp[r] = scales + m * ldg;
         zp[r] = kZeros ? zeros + m * ldg : nullptr;
     }
+    // LDS of the wave: 16 bytes of every lane on their way to another, scales and zero points of a segment
+    char* const mine = reinterpret_cast<char*>(part) + wave * w4_tile_lds(kRowTiles, kTokTiles);
+    T* const my_s = reinterpret_cast<T*>(mine + 1024);
+    unsigned char* const my_z = reinterpret_cast<unsigned char*>(my_s + kRowTiles * 16 * kW4Segment);
 #pragma unroll
-    for (int t = 0; t < kTokTiles; ++t) xp[t] = x + static_cast<int64_t>(min(t0 + t * 16 + row, batch - 1)) * ldx + quarter * 8;
+    for (int t = 0; t < kTokTiles; ++t) xp[t] = x + static_cast<int64_t>(min(t0 + t * 16 + load_row_of, batch - 1)) * ldx + load_part * 8;
 
     v4f total[kTokTiles][kRowTiles];
 #pragma unroll
@@ -292,6 +303,7 @@ __global__ __launch_bounds__(W4TW * kWave) void w4_tile_kernel(int batch, int M,
 #pragma unroll
         for (int r = 0; r < kRowTiles; ++r) total[t][r] = v4f{0.f, 0.f, 0.f, 0.f};
 
+    const nibble_maker<T> nibbles;
     // one unit: 32 columns at a time, the scale applied where a group ends
     auto unit_products = [&](const v4u (&wt)[kRowTiles], const float (&scale)[kRowTiles][kGroups], const float (&offset)[kRowTiles][kGroups],
                              const v4u (&xv)[kTokTiles][4]) {
@@ -312,7 +324,7 @@ __global__ __launch_bounds__(W4TW * kWave) void w4_tile_kernel(int batch, int M,
                 }
 #pragma unroll
                 for (int r = 0; r < kRowTiles; ++r) {
-                    const v4u wq = nibbles_plus_16<T>(wt[r][d]);
+                    const v4u wq = nibbles(wt[r][d]);
 #pragma unroll
                     for (int t = 0; t < kTokTiles; ++t) acc[t][r] = mfma_16x16x32<T>(xo[t], wq, k == 0 ? zero : acc[t][r]);
                 }
@@ -326,86 +338,122 @@ __global__ __launch_bounds__(W4TW * kWave) void w4_tile_kernel(int batch, int M,
                         total[t][r][i] = __builtin_fmaf(scale[r][g], __builtin_fmaf(-offset[r][g], sum[t][i], acc[t][r][i]), total[t][r][i]);
         }
     };
+    // Part p of row i stands at (p ^ i / 4): sixteen lanes meet no bank twice, neither writing nor reading.  A wave's LDS
+    // accesses are carried out in order, so one place does for all.
+    auto to_instruction_order = [&](v4u v) {
+        *reinterpret_cast<v4u*>(mine + load_row_of * 64 + ((load_part ^ (load_row_of >> 2)) & 3) * 16) = v;
+        __builtin_amdgcn_wave_barrier();
+        const v4u got = *reinterpret_cast<const v4u*>(mine + row * 64 + ((quarter ^ (row >> 2)) & 3) * 16);
+        __builtin_amdgcn_wave_barrier();
+        return got;
+    };
     v4u wt[kRowTiles];
     float scale[kRowTiles][kGroups], offset[kRowTiles][kGroups];
 
     if (begin < end) {
-        // Units go in pairs (begin and end are even).  Everything of a pair is requested one pair ahead and in the order of
-        // its use, since loads return in order; the scales of a pair are consecutive, one load per row.
-        typedef T pair_scales __attribute__((ext_vector_type(2 * kGroups)));
-        typedef unsigned char pair_zeros __attribute__((ext_vector_type(2 * kGroups)));
-        typedef pair_scales pair_scales_any __attribute__((aligned(2)));
-        typedef pair_zeros pair_zeros_any __attribute__((aligned(1)));
+        // Units go in pairs (begin and end are even).  Everything of a pair is requested one pair ahead, and in the order of
+        // its use, since loads return in order.
+        typedef T scales4 __attribute__((ext_vector_type(4)));
+        typedef unsigned char zeros4 __attribute__((ext_vector_type(4)));
+        typedef scales4 scales4_any __attribute__((aligned(2)));
+        typedef zeros4 zeros4_any __attribute__((aligned(1)));
+        constexpr int kSegmentUnits = kW4Segment / kGroups;
         v4u w[2][kRowTiles], xv[2][kTokTiles][4];
-        pair_scales sv[kRowTiles];
-        pair_zeros zv[kRowTiles];
-        // past the wave's last pair the loads repeat it: without a branch they stay in flight
+        scales4 sv[kRowTiles];
+        zeros4 zv[kRowTiles];
+        // four scales of the lane's row from unit u on; behind the row's last one that one again (of no use)
         auto load_scales = [&](int u) {
-            const int64_t g = static_cast<int64_t>(min(u, end - 2)) * kGroups;
+            const int g = u * kGroups + 4 * load_part;
+            const bool whole = (u + kSegmentUnits) * kGroups <= groups;  // the same for all lanes
 #pragma unroll
             for (int r = 0; r < kRowTiles; ++r) {
-                sv[r] = *reinterpret_cast<const pair_scales_any*>(sp[r] + g);
-                if (kZeros) zv[r] = *reinterpret_cast<const pair_zeros_any*>(zp[r] + g);
+                if (whole) {
+                    sv[r] = *reinterpret_cast<const scales4_any*>(sp[r] + g);
+                    if (kZeros) zv[r] = *reinterpret_cast<const zeros4_any*>(zp[r] + g);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        sv[r][i] = sp[r][min(g + i, groups - 1)];
+                        if (kZeros) zv[r][i] = zp[r][min(g + i, groups - 1)];
+                    }
+                }
             }
+            loads_start_here();
         };
+        // past the wave's last pair the loads repeat it: without a branch they stay in flight
         auto load_unit = [&](int u, int k) {
             const int64_t at = min(u, end - 2) + k;
-#pragma unroll
-            for (int r = 0; r < kRowTiles; ++r) w[k][r] = load16(reinterpret_cast<const T*>(wp[r] + at * (kW4Unit / 2)));
 #pragma unroll
             for (int t = 0; t < kTokTiles; ++t)
 #pragma unroll
                 for (int d = 0; d < 4; ++d) xv[k][t][d] = load16(xp[t] + at * kW4Unit + d * 32);
+#pragma unroll
+            for (int r = 0; r < kRowTiles; ++r) w[k][r] = load16(reinterpret_cast<const T*>(wp[r] + at * (kW4Unit / 2)));
+            loads_start_here();
         };
         load_scales(begin);
         load_unit(begin, 0);
         load_unit(begin, 1);
-        for (int u = begin; u < end; u += 2) {
-            float pair_scale[2][kRowTiles][kGroups], pair_offset[2][kRowTiles][kGroups];
+        for (int u0 = begin; u0 < end; u0 += kSegmentUnits) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int r = 0; r < kRowTiles; ++r) {
+                *reinterpret_cast<scales4*>(my_s + (r * 16 + load_row_of) * kW4Segment + 4 * load_part) = sv[r];
+                if (kZeros) *reinterpret_cast<zeros4*>(my_z + (r * 16 + load_row_of) * kW4Segment + 4 * load_part) = zv[r];
+            }
+            __builtin_amdgcn_wave_barrier();
+            load_scales(min(u0 + kSegmentUnits, end - 1));
+            for (int u = u0; u < min(end, u0 + kSegmentUnits); u += 2) {
 #pragma unroll
-                for (int r = 0; r < kRowTiles; ++r)
+                for (int k = 0; k < 2; ++k) {
+                    v4u xo[kTokTiles][4];
 #pragma unroll
-                    for (int g = 0; g < kGroups; ++g) {
-                        pair_scale[k][r][g] = static_cast<float>(sv[r][k * kGroups + g]);
-                        pair_offset[k][r][g] = 16.f + (kZeros ? static_cast<float>(zv[r][k * kGroups + g]) : 8.f);
+                    for (int t = 0; t < kTokTiles; ++t)
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) xo[t][d] = to_instruction_order(xv[k][t][d]);
+#pragma unroll
+                    for (int r = 0; r < kRowTiles; ++r) {
+                        wt[r] = transpose_quarters(to_instruction_order(w[k][r]));
+#pragma unroll
+                        for (int g = 0; g < kGroups; ++g) {
+                            const int at = (r * 16 + row) * kW4Segment + (u + k - u0) * kGroups + g;
+                            scale[r][g] = static_cast<float>(my_s[at]);
+                            offset[r][g] = 16.f + (kZeros ? static_cast<float>(my_z[at]) : 8.f);
+                        }
                     }
-            load_scales(u + 2);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-#pragma unroll
-                for (int r = 0; r < kRowTiles; ++r) wt[r] = transpose_quarters(w[k][r]);
-                unit_products(wt, pair_scale[k], pair_offset[k], xv[k]);
-                load_unit(u + 2, k);
+                    load_unit(u + 2, k);
+                    unit_products(wt, scale, offset, xo);
+                }
             }
         }
     }
     // the last, odd unit and the columns behind the last whole one, one at a time
-    for (int u = max(full & ~1, wave * units_per_wave); u < min(units, (wave + 1) * units_per_wave); ++u) {
+    for (int u = max(full & ~1, begin); u < min(units, begin + units_per_wave); ++u) {
         v4u xv[kTokTiles][4];
         const int row_bytes = (N + 1) / 2, at = u * (kW4Unit / 2) + quarter * 16;
 #pragma unroll
         for (int r = 0; r < kRowTiles; ++r) {
+            const int64_t m = row_at(r, row);
             v4u w;
 #pragma unroll
             for (int d = 0; d < 4; ++d)  // whole dwords: the last may hold bytes behind the row, whose x is zero
-                w[d] = at + 4 * d < row_bytes ? *reinterpret_cast<const unsigned*>(wp[r] + u * (kW4Unit / 2) + 4 * d) : 0u;
+                w[d] = at + 4 * d < row_bytes ? *reinterpret_cast<const unsigned*>(q + m * ldq + at + 4 * d) : 0u;
             wt[r] = transpose_quarters(w);
 #pragma unroll
             for (int g = 0; g < kGroups; ++g) {
                 const int64_t i = min(u * kGroups + g, groups - 1);  // behind the last column: x is zero
-                scale[r][g] = static_cast<float>(sp[r][i]);
-                offset[r][g] = 16.f + (kZeros ? static_cast<float>(zp[r][i]) : 8.f);
+                scale[r][g] = static_cast<float>(scales[m * ldg + i]);
+                offset[r][g] = 16.f + (kZeros ? static_cast<float>(zeros[m * ldg + i]) : 8.f);
             }
         }
 #pragma unroll
         for (int t = 0; t < kTokTiles; ++t)
 #pragma unroll
-            for (int d = 0; d < 4; ++d) xv[t][d] = load_row(xp[t] - quarter * 8, u * kW4Unit + d * 32 + quarter * 8, N);
+            for (int d = 0; d < 4; ++d)
+                xv[t][d] = load_row(x + static_cast<int64_t>(min(t0 + t * 16 + row, batch - 1)) * ldx, u * kW4Unit + d * 32 + quarter * 8, N);
         unit_products(wt, scale, offset, xv);
     }
 
+    __syncthreads();  // the waves' sums take the place of x
     constexpr int kTiles = kTokTiles * kRowTiles;
 #pragma unroll
     for (int t = 0; t < kTokTiles; ++t)
@@ -440,7 +488,40 @@ int panel_of(int N, int tb, size_t elem) {
 template <class T, bool kZeros>
 int launch_w4(int batch, int M, int N, int group_shift, float alpha, const unsigned char* q, int64_t ldq, const void* scales,
               const unsigned char* zeros, int64_t ldg, const void* x, int64_t ldx, float beta, void* y, int64_t ldy, hipStream_t stream) {
+    using std::integral_constant;
     const int cus = device_cus();
+    if constexpr (sizeof(T) == 2) {
+        auto tile = [&](auto row_tiles, auto tok_tiles, auto steps) {
+            constexpr int kRowTiles = decltype(row_tiles)::value, kTokTiles = decltype(tok_tiles)::value;
+            const int units = static_cast<int>(ceil_div(N, kW4Unit));
+            const int per_wave = static_cast<int>(ceil_div(units, 2 * kW4TileWaves)) * 2;
+            const int waves = static_cast<int>(ceil_div(units, per_wave));
+            const size_t lds = static_cast<size_t>(waves) * w4_tile_lds(kRowTiles, kTokTiles);
+            const dim3 grid(static_cast<unsigned>(ceil_div(M, 16 * kRowTiles)), static_cast<unsigned>(ceil_div(batch, 16 * kTokTiles)));
+            w4_tile_kernel<T, kRowTiles, kTokTiles, decltype(steps)::value, kZeros><<<grid, waves * kWave, lds, stream>>>(
+                batch, M, N, alpha, q, ldq, static_cast<const T*>(scales), zeros, ldg, static_cast<const T*>(x), ldx, beta,
+                static_cast<T*>(y), ldy, per_wave);
+        };
+        auto of_group = [&](auto row_tiles, auto tok_tiles) {
+            if (group_shift == 5) tile(row_tiles, tok_tiles, integral_constant<int, 1>{});
+            else if (group_shift == 6) tile(row_tiles, tok_tiles, integral_constant<int, 2>{});
+            else tile(row_tiles, tok_tiles, integral_constant<int, 4>{});
+        };
+        // Two tokens cost the other form 32 us on 16384 x 16384 and this one 35, four 45 and 36.
+        if (batch >= kW4TileTokens && N > 0) {
+            // Row tiles of a workgroup: every one of them reads all of x, which is what bounds this form (12 TB/s out of the
+            // caches), but the CUs have to be covered.  Thirteen tokens, one / two / four tiles: 4096 x 8192 9.8 / 12.3 /
+            // 17.8 us, 8192 x 8192 16.5 / 13.7 / 19.2 us, 16384 x 16384 (sixteen tokens) 58 / 43 / 39 us.
+            // (thirty-two tokens as two tiles of one workgroup: 8192 x 8192 18.1 us, as two workgroups 21.0)
+            if (batch > 16) {
+                if (M > 16 * cus) of_group(integral_constant<int, 2>{}, integral_constant<int, 2>{});
+                else of_group(integral_constant<int, 1>{}, integral_constant<int, 2>{});
+            } else if (M > 48 * cus) of_group(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+            else if (M > 16 * cus) of_group(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+            else of_group(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+            return launch_status();
+        }
+    }
     auto go = [&](auto tb, auto rows) {
         constexpr int TB = decltype(tb)::value, kRows = decltype(rows)::value, kPieces = kRows < 4 ? 4 / kRows : 1;
         const int panel = panel_of(N, TB, sizeof(T));
@@ -449,43 +530,23 @@ int launch_w4(int batch, int M, int N, int group_shift, float alpha, const unsig
         int waves = kW4MaxWaves;
         while (waves > 4 && ceil_div(M, waves * kRows) < cus) waves /= 2;
         const int unit = waves * kRows;
-        const int per_block = static_cast<int>(ceil_div(ceil_div(M, unit), cus * (W4BPC))) * unit;
+        // x in several panels is staged for every round of rows: one round per workgroup then
+        const int per_block = panel < N ? unit : static_cast<int>(ceil_div(ceil_div(M, unit), cus)) * unit;
         const dim3 grid(static_cast<unsigned>(ceil_div(M, per_block)), static_cast<unsigned>(ceil_div(batch, TB)));
         w4_gemv_kernel<T, TB, kRows, kPieces, kZeros><<<grid, waves * kWave, lds, stream>>>(
             batch, M, N, group_shift, alpha, q, ldq, static_cast<const T*>(scales), zeros, ldg, static_cast<const T*>(x), ldx, beta,
             static_cast<T*>(y), ldy, per_block, panel);
     };
-    using std::integral_constant;
-    if constexpr (sizeof(T) == 2)
-        if (batch >= W4MIN && N > 0) {
-            auto tile = [&](auto row_tiles, auto tok_tiles) {
-                constexpr int kRowTiles = decltype(row_tiles)::value, kTokTiles = decltype(tok_tiles)::value;
-                const int units = static_cast<int>(ceil_div(N, kW4Unit));
-                const int per_wave = static_cast<int>(ceil_div(units, 2 * W4TW)) * 2;
-                const int waves = static_cast<int>(ceil_div(units, per_wave));
-                const size_t lds = static_cast<size_t>(waves) * kRowTiles * kTokTiles * 4 * kWave * sizeof(float);
-                const dim3 grid(static_cast<unsigned>(ceil_div(M, 16 * kRowTiles)), static_cast<unsigned>(ceil_div(batch, 16 * kTokTiles)));
-                auto of_group = [&](auto steps) {
-                w4_tile_kernel<T, kRowTiles, kTokTiles, decltype(steps)::value, kZeros><<<grid, waves * kWave, lds, stream>>>(
-                    batch, M, N, alpha, q, ldq, static_cast<const T*>(scales), zeros, ldg, static_cast<const T*>(x), ldx, beta,
-                    static_cast<T*>(y), ldy, per_wave);
-                };
-                if (group_shift == 5) of_group(integral_constant<int, 1>{});
-                else if (group_shift == 6) of_group(integral_constant<int, 2>{});
-                else of_group(integral_constant<int, 4>{});
-            };
-            tile(integral_constant<int, W4RT>{}, integral_constant<int, 1>{});
-            return launch_status();
-        }
-    // rows per wave and step: as many as leave every CU its sixteen waves
-    auto by_rows = [&](auto tb) {
-        if (M >= 64 * cus W4ROWS) go(tb, integral_constant<int, 4>{});
-        else if (M >= 32 * cus W4ROWS) go(tb, integral_constant<int, 2>{});
+    // Rows per wave and step: as many as leave every CU its sixteen waves.  Four FP32 tokens take x in panels, staged anew for
+    // every round of rows, so there two rows pay earlier: seven tokens by 6143 x 8201 41 us, with one row 56.
+    auto by_rows = [&](auto tb, int two_rows_from) {
+        if (M >= 64 * cus) go(tb, integral_constant<int, 4>{});
+        else if (M >= two_rows_from * cus) go(tb, integral_constant<int, 2>{});
         else go(tb, integral_constant<int, 1>{});
     };
-    if (batch == 1) by_rows(integral_constant<int, 1>{});
-    else if (batch == 2) by_rows(integral_constant<int, 2>{});
-    else by_rows(integral_constant<int, 4>{});
+    if (batch == 1) by_rows(integral_constant<int, 1>{}, 32);
+    else if (batch == 2 || sizeof(T) == 2) by_rows(integral_constant<int, 2>{}, 32);
+    else if constexpr (sizeof(T) == 4) by_rows(integral_constant<int, 4>{}, 16);
     return launch_status();
 }
 
