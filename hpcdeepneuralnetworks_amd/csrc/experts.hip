@@ -15,9 +15,17 @@ namespace hpcdnn {
 
 // ---- sort -----------------------------------------------------------------
 
-constexpr int kSortThreads = 1024;
-constexpr int kSortMaxBlocks = 256;
-constexpr int kSortMinSlots = 4096;  // slots of a workgroup; up to this many are sorted by one workgroup in one launch
+constexpr int kSortMaxThreads = 1024;
+constexpr int kSortOneBlock = 4096;  // slots up to which one workgroup sorts them in one launch
+constexpr int kSortMinSlots = 1024;  // slots of a workgroup beyond that, more where there would be over kSortMaxBlocks
+constexpr int kSortMaxBlocks = 128;  // (every one of them reads the counts of all)
+
+// Expert of slot s; slots of a row-contiguous list lie one after the other, and the division is spared.
+__device__ __forceinline__ int expert_of(const int* __restrict__ ids, int64_t ldids, unsigned s, unsigned topk) {
+    if (ldids == topk) return ids[s];
+    const unsigned t = s / topk;
+    return ids[t * ldids + (s - t * topk)];
+}
 
 // Lanes of the wave that hold the same key as this one, among those with `on`: one ballot per bit of the key.
 __device__ __forceinline__ uint64_t same_key(int key, bool on, int bits) {
@@ -30,61 +38,64 @@ __device__ __forceinline__ uint64_t same_key(int key, bool on, int bits) {
 }
 
 // counts[block][e] = slots of the workgroup's chunk that go to expert e
-__global__ __launch_bounds__(kSortThreads) void expert_count_kernel(int64_t slots, int per_block, int topk, int experts,
-                                                                    const int* __restrict__ ids, int64_t ldids, int* __restrict__ counts) {
-    extern __shared__ int hist[];  // [experts]
-    for (int e = threadIdx.x; e < experts; e += kSortThreads) hist[e] = 0;
+__global__ __launch_bounds__(kSortMaxThreads) void expert_count_kernel(unsigned slots, unsigned per_block, int topk, int experts,
+                                                                       const int* __restrict__ ids, int64_t ldids, int* __restrict__ counts) {
+    __shared__ int hist[HPCDNN_EXPERTS_MAX];
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) hist[e] = 0;
     __syncthreads();
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block, last = min(slots, first + per_block);
-    for (int64_t s = first + threadIdx.x; s < last; s += kSortThreads) {
-        const int t = static_cast<int>(s / topk);
-        const int id = ids[t * ldids + (s - static_cast<int64_t>(t) * topk)];
+    const unsigned first = blockIdx.x * per_block, last = min(slots, first + per_block);
+    for (unsigned s = first + threadIdx.x; s < last; s += blockDim.x) {
+        const int id = expert_of(ids, ldids, s, topk);
         if (id >= 0 && id < experts) atomicAdd(&hist[id], 1);
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += kSortThreads) counts[static_cast<int64_t>(blockIdx.x) * experts + e] = hist[e];
+    for (int e = threadIdx.x; e < experts; e += blockDim.x) counts[blockIdx.x * experts + e] = hist[e];
 }
 
 // Places of the workgroup's slots.  Every workgroup adds up the counts of all workgroups by itself (they come from L2), so
 // there is no launch for a scan; counts == nullptr: one workgroup has all the slots.  Within the workgroup each wave has a
 // run of consecutive slots: it counts them per expert, the counts are scanned over waves, and in a second walk a slot's
-// place is the wave's next place for its expert plus the number of earlier lanes with the same expert.
-__global__ __launch_bounds__(kSortThreads) void expert_place_kernel(int64_t slots, int per_block, int topk, int experts, int bits,
-                                                                    const int* __restrict__ ids, int64_t ldids,
-                                                                    const int* __restrict__ counts, int blocks, int* __restrict__ offsets,
-                                                                    int* __restrict__ pos, int* __restrict__ order) {
+// place is the wave's next place for its expert plus the number of earlier lanes with the same expert.  Integer sums only,
+// so the order of the LDS additions does not show.  The workgroup has at least as many threads as there are experts.
+__global__ __launch_bounds__(kSortMaxThreads) void expert_place_kernel(unsigned slots, unsigned per_block, int topk, int experts, int bits,
+                                                                       const int* __restrict__ ids, int64_t ldids,
+                                                                       const int* __restrict__ counts, int blocks, int* __restrict__ offsets,
+                                                                       int* __restrict__ pos, int* __restrict__ order) {
     extern __shared__ int lds[];
-    const int waves = kSortThreads / kWave;
+    const int waves = blockDim.x / kWave;
     int* next = lds;                          // [waves][experts] counts, then next places
     int* before = lds + waves * experts;      // [experts] slots of earlier workgroups
-    int* total = before + experts;            // [experts] slots of all workgroups, then first places
-    __shared__ int wave_total[kSortThreads / kWave];
+    int* total = before + experts;            // [experts] slots of all workgroups
+    __shared__ int wave_total[kSortMaxThreads / kWave];
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    for (int i = threadIdx.x; i < (waves + 2) * experts; i += kSortThreads) lds[i] = 0;
+    const unsigned first = blockIdx.x * per_block, last = min(slots, first + per_block);
+    const unsigned per_wave = per_block / waves;  // a multiple of 64
+    const unsigned begin = first + wave * per_wave, end = min(last, begin + per_wave);
+    // the first 64 slots' experts are on their way while LDS is cleared
+    int id0 = begin + lane < end ? expert_of(ids, ldids, begin + lane, topk) : -1;
+    for (int i = threadIdx.x; i < (waves + 2) * experts; i += blockDim.x) lds[i] = 0;
     __syncthreads();
-
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * per_block, last = min(slots, first + per_block);
-    const int per_wave = per_block / waves;  // a multiple of 64
-    const int64_t begin = first + static_cast<int64_t>(wave) * per_wave, end = min(last, begin + per_wave);
-    auto key_of = [&](int64_t s) {
-        const int t = static_cast<int>(s / topk);
-        return ids[t * ldids + (s - static_cast<int64_t>(t) * topk)];
-    };
-    for (int64_t s = begin + lane; s < end; s += kWave) {
-        const int id = key_of(s);
+    if (id0 >= 0 && id0 < experts) atomicAdd(&next[wave * experts + id0], 1);
+    for (unsigned s = begin + kWave + lane; s < end; s += kWave) {
+        const int id = expert_of(ids, ldids, s, topk);
         if (id >= 0 && id < experts) atomicAdd(&next[wave * experts + id], 1);
     }
-    // earlier workgroups' and all workgroups' slots per expert: threads (expert, share of the workgroups)
-    if (counts != nullptr)
-        for (int64_t i = threadIdx.x; i < static_cast<int64_t>(blocks) * experts; i += kSortThreads) {
-            const int e = static_cast<int>(i % experts), c = counts[i];
-            if (c != 0) {
-                if (i / experts < static_cast<int64_t>(blockIdx.x)) atomicAdd(&before[e], c);
-                atomicAdd(&total[e], c);
+    if (counts != nullptr) {
+        // threads (share of the workgroups, expert)
+        const int e = threadIdx.x & ((1 << bits) - 1), shares = blockDim.x >> bits, share = threadIdx.x >> bits;
+        if (e < experts && share < shares) {
+            int all = 0, earlier = 0;
+            for (int b = share; b < blocks; b += shares) {
+                const int c = counts[b * experts + e];
+                all += c;
+                if (b < static_cast<int>(blockIdx.x)) earlier += c;
             }
+            atomicAdd(&total[e], all);
+            atomicAdd(&before[e], earlier);
         }
+    }
     __syncthreads();
-    // exclusive scan of the totals over the experts (at most one per thread), and of the waves' counts
+    // exclusive scan of the totals over the experts, one per thread, and of the waves' counts
     const int e = threadIdx.x;
     int mine = 0;
     if (e < experts) {
@@ -114,9 +125,9 @@ __global__ __launch_bounds__(kSortThreads) void expert_place_kernel(int64_t slot
         }
     }
     __syncthreads();
-    for (int64_t s0 = begin; s0 < end; s0 += kWave) {
-        const int64_t s = s0 + lane;
-        const int id = s < end ? key_of(s) : -1;
+    for (unsigned s0 = begin; s0 < end; s0 += kWave) {
+        const unsigned s = s0 + lane;
+        const int id = s0 == begin ? id0 : s < end ? expert_of(ids, ldids, s, topk) : -1;
         const bool sent = id >= 0 && id < experts;
         const uint64_t peers = same_key(id, sent, bits);
         const int rank = __popcll(peers & ((1ull << lane) - 1));
@@ -261,13 +272,17 @@ __global__ __launch_bounds__(kRowThreads) void expert_combine_grad_kernel(int to
 namespace {
 
 struct sort_plan {
-    int blocks, per_block;
+    int blocks, threads;
+    unsigned per_block;  // slots, a multiple of the threads
 };
-// Workgroups of kSortMinSlots slots, of more when that would be more than kSortMaxBlocks (every workgroup reads all counts).
-sort_plan plan_sort(int64_t slots) {
-    const int64_t unit = kSortThreads;
-    int64_t per = std::max<int64_t>(kSortMinSlots, ceil_div(ceil_div(slots, kSortMaxBlocks), unit) * unit);
-    return {static_cast<int>(std::max<int64_t>(1, ceil_div(slots, per))), static_cast<int>(per)};
+sort_plan plan_sort(int64_t slots, int experts) {
+    if (slots <= kSortOneBlock) {
+        // a wave per 64 slots up to sixteen, four at least and as many as the scan over the experts needs
+        const int threads = static_cast<int>(std::min<int64_t>(kSortMaxThreads, std::max<int64_t>({ceil_div(slots, kWave), ceil_div(experts, kWave), 4}) * kWave));
+        return {1, threads, static_cast<unsigned>(std::max<int64_t>(1, ceil_div(slots, threads)) * threads)};
+    }
+    const int64_t per = std::max<int64_t>(kSortMinSlots, ceil_div(ceil_div(slots, kSortMaxBlocks), kSortMaxThreads) * kSortMaxThreads);
+    return {static_cast<int>(ceil_div(slots, per)), kSortMaxThreads, static_cast<unsigned>(per)};
 }
 
 bool choices_valid(int tokens, int topk) {
@@ -292,7 +307,7 @@ int token_grid(int tokens) { return std::min(tokens, 1 << 20); }
 
 size_t expert_sort_workspace_bytes(int tokens, int topk, int experts) {
     if (!choices_valid(tokens, topk) || experts < 1 || experts > HPCDNN_EXPERTS_MAX) return 0;
-    const sort_plan p = plan_sort(static_cast<int64_t>(tokens) * topk);
+    const sort_plan p = plan_sort(static_cast<int64_t>(tokens) * topk, experts);
     return p.blocks > 1 ? static_cast<size_t>(p.blocks) * experts * sizeof(int) : 0;
 }
 
@@ -306,7 +321,7 @@ extern "C" int hpcdnn_expert_sort(int tokens, int topk, int experts, const int32
     if (tokens > 0 && (ids == nullptr || ldids < topk || pos == nullptr || !aligned(ids, 4) || !aligned(pos, 4) || !aligned(order, 4)))
         return HPCDNN_ERR_INVALID_VALUE;
     const int64_t slots = static_cast<int64_t>(tokens) * topk;
-    const sort_plan p = plan_sort(slots);
+    const sort_plan p = plan_sort(slots, experts);
     if (p.blocks > 1) {
         if (!aligned(ws, 16)) return HPCDNN_ERR_INVALID_VALUE;
         if (ws == nullptr || ws_bytes < expert_sort_workspace_bytes(tokens, topk, experts)) return HPCDNN_ERR_WORKSPACE;
@@ -314,14 +329,14 @@ extern "C" int hpcdnn_expert_sort(int tokens, int topk, int experts, const int32
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     int bits = 0;
     while ((1 << bits) < experts) ++bits;
-    const size_t lds = static_cast<size_t>(kSortThreads / kWave + 2) * experts * sizeof(int);
+    const size_t lds = static_cast<size_t>(p.threads / kWave + 2) * experts * sizeof(int);
     int* counts = nullptr;
     if (p.blocks > 1) {
         counts = static_cast<int*>(ws);
-        expert_count_kernel<<<p.blocks, kSortThreads, experts * sizeof(int), stream>>>(slots, p.per_block, topk, experts, ids, ldids, counts);
+        expert_count_kernel<<<p.blocks, p.threads, 0, stream>>>(static_cast<unsigned>(slots), p.per_block, topk, experts, ids, ldids, counts);
     }
-    expert_place_kernel<<<p.blocks, kSortThreads, lds, stream>>>(slots, p.per_block, topk, experts, bits, ids, ldids, counts, p.blocks,
-                                                                 offsets, pos, order);
+    expert_place_kernel<<<p.blocks, p.threads, lds, stream>>>(static_cast<unsigned>(slots), p.per_block, topk, experts, bits, ids, ldids,
+                                                              counts, p.blocks, offsets, pos, order);
     return launch_status();
 }
 

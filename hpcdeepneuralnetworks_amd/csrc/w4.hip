@@ -114,7 +114,7 @@ __global__ __launch_bounds__(kW4MaxWaves * kWave) void w4_gemv_kernel(int batch,
 #pragma unroll
             for (int u = 0; u < kPieces; ++u) {
                 const int col = n0 + (p0 + u) * kW4Piece + lane * kW4Cols;
-                w[r][u] = __builtin_amdgcn_raw_buffer_load_b128(rs, col / 2, 0, 0);
+                w[r][u] = __builtin_amdgcn_raw_buffer_load_b128(rs, col / 2, 0, 2);  // non-temporal: read once (4 % faster)
                 const int64_t g = at * ldg + (min(col, N - 1) >> group_shift);  // behind the last column: x is zero
                 s[r][u] = scales[g];
                 if (kZeros) z[r][u] = zeros[g];
