@@ -206,3 +206,24 @@ def test_wrappers_refuse_host_tensors_and_mixed_types():
     with pytest.raises(blas.HpcdnnError):
         blas._param_type((torch.zeros(8), torch.zeros(8, dtype=torch.float16)), torch.float16)
     assert blas._param_type((None, torch.zeros(8)), torch.float16) == torch.float32
+
+
+def test_wrappers_refuse_a_tensor_of_another_device(monkeypatch):
+    """What a call enqueues goes to the current device's stream: an operand that lives elsewhere is refused."""
+    from hpcdeepneuralnetworks_amd import blas
+
+    class Elsewhere(torch.Tensor):
+        is_cuda = True
+        device = torch.device("cuda", 1)
+
+        def get_device(self):
+            return 1
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    x = torch.zeros(4, 8).as_subclass(Elsewhere)
+    with pytest.raises(blas.HpcdnnError, match="not the current device"):
+        blas.layer_norm(4, 8, x, None, None, 1e-5, x)
+    with pytest.raises(blas.HpcdnnError, match="not the current device"):
+        blas.expert_gather(4, 1, 4, 8, x, x, x)
+    with pytest.raises(blas.HpcdnnError, match="current device"):
+        blas._scratch(x, 0)
