@@ -233,9 +233,14 @@ __global__ __launch_bounds__(kW4MaxWaves * kWave) void w4_gemv_kernel(int batch,
 // stays inside one group.  The sums over x that take out the offset of the nibbles come from the same instruction with a
 // matrix of ones.
 constexpr int kW4Unit = 128;
-constexpr int kW4TileTokens = 3;  // tokens from which this form is taken
+// Tokens from which this form is taken.  16-bit: two cost the other form 32 us on 16384 x 16384 and this one 35, four 45 and 36.
+// FP32 (instructions of four columns, an eighth of the rate): four by 8192 x 8192 22 and 31 us, seven by 6143 x 8201 48 and 37.
+template <class T>
+constexpr int kW4TileTokens = sizeof(T) == 2 ? 3 : 5;
 constexpr int kW4TileWaves = 8;
 constexpr int kW4Segment = 16;  // scales of a row that a wave keeps in LDS at a time
+template <class T>
+constexpr int kW4Exchange = kWave * 32 * static_cast<int>(sizeof(T)) / 4 / 2;  // 8 values of every lane: 1 or 2 KiB
 
 typedef f16 v8h __attribute__((ext_vector_type(8)));
 typedef bf16 v8b __attribute__((ext_vector_type(8)));
@@ -257,8 +262,9 @@ __device__ __forceinline__ v4u transpose_quarters(v4u w) {
 }
 
 // LDS of a wave of the kernel below: its parts, or its sums at the end.
+template <class T>
 constexpr int w4_tile_lds(int row_tiles, int tok_tiles) {
-    const int parts = 1024 + row_tiles * 16 * kW4Segment * 3, sums = row_tiles * tok_tiles * 4 * kWave * 4;
+    const int parts = kW4Exchange<T> + row_tiles * 16 * kW4Segment * (static_cast<int>(sizeof(T)) + 1), sums = row_tiles * tok_tiles * 4 * kWave * 4;
     return parts > sums ? parts : sums;
 }
 
@@ -268,8 +274,10 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
                                                                        const T* __restrict__ scales, const unsigned char* __restrict__ zeros,
                                                                        int64_t ldg, const T* __restrict__ x, int64_t ldx, float beta,
                                                                        T* __restrict__ y, int64_t ldy, int units_per_wave) {
-    extern __shared__ __align__(16) float part[];  // x of a unit per wave, at the end sums [wave][tile][4][lane]
+    extern __shared__ __align__(16) float part[];  // the waves' own parts, at the end their sums [wave][tile][4][lane]
     constexpr int kGroup = 32 * kGroupSteps, kGroups = 4 / kGroupSteps;  // columns of a group, groups of a unit
+    constexpr bool kF32 = std::is_same_v<T, float>;
+    constexpr int kXParts = kF32 ? 8 : 4;          // 16-byte parts of x that a lane has of a unit
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int waves = blockDim.x / kWave;
     const int row = lane & 15, quarter = lane >> 4;
@@ -291,11 +299,11 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
         zp[r] = kZeros ? zeros + m * ldg : nullptr;
     }
     // LDS of the wave: 16 bytes of every lane on their way to another, scales and zero points of a segment
-    char* const mine = reinterpret_cast<char*>(part) + wave * w4_tile_lds(kRowTiles, kTokTiles);
-    T* const my_s = reinterpret_cast<T*>(mine + 1024);
+    char* const mine = reinterpret_cast<char*>(part) + wave * w4_tile_lds<T>(kRowTiles, kTokTiles);
+    T* const my_s = reinterpret_cast<T*>(mine + kW4Exchange<T>);
     unsigned char* const my_z = reinterpret_cast<unsigned char*>(my_s + kRowTiles * 16 * kW4Segment);
 #pragma unroll
-    for (int t = 0; t < kTokTiles; ++t) xp[t] = x + static_cast<int64_t>(min(t0 + t * 16 + load_row_of, batch - 1)) * ldx + load_part * 8;
+    for (int t = 0; t < kTokTiles; ++t) xp[t] = x + static_cast<int64_t>(min(t0 + t * 16 + load_row_of, batch - 1)) * ldx + load_part * kVec<T>;
 
     v4f total[kTokTiles][kRowTiles];
 #pragma unroll
@@ -303,30 +311,52 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
 #pragma unroll
         for (int r = 0; r < kRowTiles; ++r) total[t][r] = v4f{0.f, 0.f, 0.f, 0.f};
 
-    const nibble_maker<T> nibbles;
+    [[maybe_unused]] const nibble_maker<std::conditional_t<kF32, f16, T>> nibbles;
     // one unit: 32 columns at a time, the scale applied where a group ends
     auto unit_products = [&](const v4u (&wt)[kRowTiles], const float (&scale)[kRowTiles][kGroups], const float (&offset)[kRowTiles][kGroups],
-                             const v4u (&xv)[kTokTiles][4]) {
-        constexpr unsigned kOne = std::is_same_v<T, f16> ? 0x3C003C00u : 0x3F803F80u;
-        const v4u ones = {kOne, kOne, kOne, kOne};
+                             const v4u (&xv)[kTokTiles][kXParts]) {
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
-            v4f acc[kTokTiles][kRowTiles], sum[kTokTiles];
+            v4f acc[kTokTiles][kRowTiles];
+            [[maybe_unused]] v4f sum[kTokTiles];
 #pragma unroll
-            for (int k = 0; k < kGroupSteps; ++k) {
-                const int d = g * kGroupSteps + k;
-                const v4f zero = {0.f, 0.f, 0.f, 0.f};
-                v4u xo[kTokTiles];
+            for (int t = 0; t < kTokTiles; ++t) {
+                sum[t] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int t = 0; t < kTokTiles; ++t) {
-                    xo[t] = pair_order(xv[t][d]);
-                    sum[t] = mfma_16x16x32<T>(xo[t], ones, k == 0 ? zero : sum[t]);
-                }
+                for (int r = 0; r < kRowTiles; ++r) acc[t][r] = v4f{0.f, 0.f, 0.f, 0.f};
+            }
 #pragma unroll
-                for (int r = 0; r < kRowTiles; ++r) {
-                    const v4u wq = nibbles(wt[r][d]);
+            for (int d = g * kGroupSteps; d < (g + 1) * kGroupSteps; ++d) {
+                if constexpr (kF32) {
+                    // eight instructions of four columns each, column 32 d + 8 (l / 16) + j; q - z is exact
 #pragma unroll
-                    for (int t = 0; t < kTokTiles; ++t) acc[t][r] = mfma_16x16x32<T>(xo[t], wq, k == 0 ? zero : acc[t][r]);
+                    for (int r = 0; r < kRowTiles; ++r) {
+                        const unsigned even = wt[r][d] & 0x0f0f0f0fu, odd = (wt[r][d] >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const float wj = static_cast<float>((((j & 1) ? odd : even) >> (8 * (j / 2))) & 0xffu) - offset[r][g];
+#pragma unroll
+                            for (int t = 0; t < kTokTiles; ++t) {
+                                const float xj = __builtin_bit_cast(float, static_cast<unsigned>(xv[t][2 * d + j / 4][j & 3]));
+                                acc[t][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(xj, wj, acc[t][r], 0, 0, 0);
+                            }
+                        }
+                    }
+                } else {
+                    constexpr unsigned kOne = std::is_same_v<T, f16> ? 0x3C003C00u : 0x3F803F80u;
+                    const v4u ones = {kOne, kOne, kOne, kOne};
+                    v4u xo[kTokTiles];
+#pragma unroll
+                    for (int t = 0; t < kTokTiles; ++t) {
+                        xo[t] = pair_order(xv[t][d]);
+                        sum[t] = mfma_16x16x32<T>(xo[t], ones, sum[t]);
+                    }
+#pragma unroll
+                    for (int r = 0; r < kRowTiles; ++r) {
+                        const v4u wq = nibbles(wt[r][d]);
+#pragma unroll
+                        for (int t = 0; t < kTokTiles; ++t) acc[t][r] = mfma_16x16x32<T>(xo[t], wq, acc[t][r]);
+                    }
                 }
             }
 #pragma unroll
@@ -334,8 +364,10 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
 #pragma unroll
                 for (int t = 0; t < kTokTiles; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        total[t][r][i] = __builtin_fmaf(scale[r][g], __builtin_fmaf(-offset[r][g], sum[t][i], acc[t][r][i]), total[t][r][i]);
+                    for (int i = 0; i < 4; ++i) {
+                        const float dot = kF32 ? acc[t][r][i] : __builtin_fmaf(-offset[r][g], sum[t][i], acc[t][r][i]);
+                        total[t][r][i] = __builtin_fmaf(scale[r][g], dot, total[t][r][i]);
+                    }
         }
     };
     // Part p of row i stands at (p ^ i / 4): sixteen lanes meet no bank twice, neither writing nor reading.  A wave's LDS
@@ -347,6 +379,19 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
         __builtin_amdgcn_wave_barrier();
         return got;
     };
+    // FP32: the eight parts of a step's 32 columns, of which a lane wants parts 2 (l / 16) and the next; part p of token i at
+    // (p ^ i / 2 % 8).
+    [[maybe_unused]] auto to_instruction_order2 = [&](v4u lo, v4u hi, v4u& first, v4u& second) {
+        char* const put = mine + load_row_of * 128;
+        const int put_at = (load_row_of >> 1) & 7, get_at = (row >> 1) & 7;
+        *reinterpret_cast<v4u*>(put + (load_part ^ put_at) * 16) = lo;
+        *reinterpret_cast<v4u*>(put + ((load_part + 4) ^ put_at) * 16) = hi;
+        __builtin_amdgcn_wave_barrier();
+        first = *reinterpret_cast<const v4u*>(mine + row * 128 + ((2 * quarter) ^ get_at) * 16);
+        second = *reinterpret_cast<const v4u*>(mine + row * 128 + ((2 * quarter + 1) ^ get_at) * 16);
+        __builtin_amdgcn_wave_barrier();
+    };
+    constexpr float kOffset = kF32 ? 0.f : 16.f;   // what stands on a weight beside its zero point
     v4u wt[kRowTiles];
     float scale[kRowTiles][kGroups], offset[kRowTiles][kGroups];
 
@@ -358,7 +403,7 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
         typedef scales4 scales4_any __attribute__((aligned(2)));
         typedef zeros4 zeros4_any __attribute__((aligned(1)));
         constexpr int kSegmentUnits = kW4Segment / kGroups;
-        v4u w[2][kRowTiles], xv[2][kTokTiles][4];
+        v4u w[2][kRowTiles], xv[2][kTokTiles][kXParts];
         scales4 sv[kRowTiles];
         zeros4 zv[kRowTiles];
         // four scales of the lane's row from unit u on; behind the row's last one that one again (of no use)
@@ -386,7 +431,7 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
 #pragma unroll
             for (int t = 0; t < kTokTiles; ++t)
 #pragma unroll
-                for (int d = 0; d < 4; ++d) xv[k][t][d] = load16(xp[t] + at * kW4Unit + d * 32);
+                for (int i = 0; i < kXParts; ++i) xv[k][t][i] = load16(xp[t] + at * kW4Unit + i * 4 * kVec<T>);
 #pragma unroll
             for (int r = 0; r < kRowTiles; ++r) w[k][r] = load16(reinterpret_cast<const T*>(wp[r] + at * (kW4Unit / 2)));
             loads_start_here();
@@ -405,11 +450,14 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
             for (int u = u0; u < min(end, u0 + kSegmentUnits); u += 2) {
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    v4u xo[kTokTiles][4];
+                    v4u xo[kTokTiles][kXParts];
 #pragma unroll
                     for (int t = 0; t < kTokTiles; ++t)
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) xo[t][d] = to_instruction_order(xv[k][t][d]);
+                        for (int d = 0; d < 4; ++d) {
+                            if constexpr (kF32) to_instruction_order2(xv[k][t][2 * d], xv[k][t][2 * d + 1], xo[t][2 * d], xo[t][2 * d + 1]);
+                            else xo[t][d] = to_instruction_order(xv[k][t][d]);
+                        }
 #pragma unroll
                     for (int r = 0; r < kRowTiles; ++r) {
                         wt[r] = transpose_quarters(to_instruction_order(w[k][r]));
@@ -417,7 +465,7 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
                         for (int g = 0; g < kGroups; ++g) {
                             const int at = (r * 16 + row) * kW4Segment + (u + k - u0) * kGroups + g;
                             scale[r][g] = static_cast<float>(my_s[at]);
-                            offset[r][g] = 16.f + (kZeros ? static_cast<float>(my_z[at]) : 8.f);
+                            offset[r][g] = kOffset + (kZeros ? static_cast<float>(my_z[at]) : 8.f);
                         }
                     }
                     load_unit(u + 2, k);
@@ -428,7 +476,7 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
     }
     // the last, odd unit and the columns behind the last whole one, one at a time
     for (int u = max(full & ~1, begin); u < min(units, begin + units_per_wave); ++u) {
-        v4u xv[kTokTiles][4];
+        v4u xv[kTokTiles][kXParts];
         const int row_bytes = (N + 1) / 2, at = u * (kW4Unit / 2) + quarter * 16;
 #pragma unroll
         for (int r = 0; r < kRowTiles; ++r) {
@@ -442,14 +490,16 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
             for (int g = 0; g < kGroups; ++g) {
                 const int64_t i = min(u * kGroups + g, groups - 1);  // behind the last column: x is zero
                 scale[r][g] = static_cast<float>(scales[m * ldg + i]);
-                offset[r][g] = 16.f + (kZeros ? static_cast<float>(zeros[m * ldg + i]) : 8.f);
+                offset[r][g] = kOffset + (kZeros ? static_cast<float>(zeros[m * ldg + i]) : 8.f);
             }
         }
 #pragma unroll
         for (int t = 0; t < kTokTiles; ++t)
 #pragma unroll
-            for (int d = 0; d < 4; ++d)
-                xv[t][d] = load_row(x + static_cast<int64_t>(min(t0 + t * 16 + row, batch - 1)) * ldx, u * kW4Unit + d * 32 + quarter * 8, N);
+            for (int i = 0; i < kXParts; ++i) {
+                const int col = u * kW4Unit + (kF32 ? (i / 2) * 32 + quarter * 8 + (i & 1) * 4 : i * 32 + quarter * 8);
+                xv[t][i] = load_row(x + static_cast<int64_t>(min(t0 + t * 16 + row, batch - 1)) * ldx, col, N);
+            }
         unit_products(wt, scale, offset, xv);
     }
 
@@ -490,37 +540,35 @@ int launch_w4(int batch, int M, int N, int group_shift, float alpha, const unsig
               const unsigned char* zeros, int64_t ldg, const void* x, int64_t ldx, float beta, void* y, int64_t ldy, hipStream_t stream) {
     using std::integral_constant;
     const int cus = device_cus();
-    if constexpr (sizeof(T) == 2) {
-        auto tile = [&](auto row_tiles, auto tok_tiles, auto steps) {
-            constexpr int kRowTiles = decltype(row_tiles)::value, kTokTiles = decltype(tok_tiles)::value;
-            const int units = static_cast<int>(ceil_div(N, kW4Unit));
-            const int per_wave = static_cast<int>(ceil_div(units, 2 * kW4TileWaves)) * 2;
-            const int waves = static_cast<int>(ceil_div(units, per_wave));
-            const size_t lds = static_cast<size_t>(waves) * w4_tile_lds(kRowTiles, kTokTiles);
-            const dim3 grid(static_cast<unsigned>(ceil_div(M, 16 * kRowTiles)), static_cast<unsigned>(ceil_div(batch, 16 * kTokTiles)));
-            w4_tile_kernel<T, kRowTiles, kTokTiles, decltype(steps)::value, kZeros><<<grid, waves * kWave, lds, stream>>>(
-                batch, M, N, alpha, q, ldq, static_cast<const T*>(scales), zeros, ldg, static_cast<const T*>(x), ldx, beta,
-                static_cast<T*>(y), ldy, per_wave);
-        };
-        auto of_group = [&](auto row_tiles, auto tok_tiles) {
-            if (group_shift == 5) tile(row_tiles, tok_tiles, integral_constant<int, 1>{});
-            else if (group_shift == 6) tile(row_tiles, tok_tiles, integral_constant<int, 2>{});
-            else tile(row_tiles, tok_tiles, integral_constant<int, 4>{});
-        };
-        // Two tokens cost the other form 32 us on 16384 x 16384 and this one 35, four 45 and 36.
-        if (batch >= kW4TileTokens && N > 0) {
-            // Row tiles of a workgroup: every one of them reads all of x, which is what bounds this form (12 TB/s out of the
-            // caches), but the CUs have to be covered.  Thirteen tokens, one / two / four tiles: 4096 x 8192 9.8 / 12.3 /
-            // 17.8 us, 8192 x 8192 16.5 / 13.7 / 19.2 us, 16384 x 16384 (sixteen tokens) 58 / 43 / 39 us.
-            // (thirty-two tokens as two tiles of one workgroup: 8192 x 8192 18.1 us, as two workgroups 21.0)
-            if (batch > 16) {
-                if (M > 16 * cus) of_group(integral_constant<int, 2>{}, integral_constant<int, 2>{});
-                else of_group(integral_constant<int, 1>{}, integral_constant<int, 2>{});
-            } else if (M > 48 * cus) of_group(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-            else if (M > 16 * cus) of_group(integral_constant<int, 2>{}, integral_constant<int, 1>{});
-            else of_group(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-            return launch_status();
-        }
+    auto tile = [&](auto row_tiles, auto tok_tiles, auto steps) {
+        constexpr int kRowTiles = decltype(row_tiles)::value, kTokTiles = decltype(tok_tiles)::value;
+        const int units = static_cast<int>(ceil_div(N, kW4Unit));
+        const int per_wave = static_cast<int>(ceil_div(units, 2 * kW4TileWaves)) * 2;
+        const int waves = static_cast<int>(ceil_div(units, per_wave));
+        const size_t lds = static_cast<size_t>(waves) * w4_tile_lds<T>(kRowTiles, kTokTiles);
+        const dim3 grid(static_cast<unsigned>(ceil_div(M, 16 * kRowTiles)), static_cast<unsigned>(ceil_div(batch, 16 * kTokTiles)));
+        w4_tile_kernel<T, kRowTiles, kTokTiles, decltype(steps)::value, kZeros><<<grid, waves * kWave, lds, stream>>>(
+            batch, M, N, alpha, q, ldq, static_cast<const T*>(scales), zeros, ldg, static_cast<const T*>(x), ldx, beta, static_cast<T*>(y),
+            ldy, per_wave);
+    };
+    auto of_group = [&](auto row_tiles, auto tok_tiles) {
+        if (group_shift == 5) tile(row_tiles, tok_tiles, integral_constant<int, 1>{});
+        else if (group_shift == 6) tile(row_tiles, tok_tiles, integral_constant<int, 2>{});
+        else tile(row_tiles, tok_tiles, integral_constant<int, 4>{});
+    };
+    if (batch >= kW4TileTokens<T> && N > 0) {
+        // Row tiles of a workgroup: every one of them reads all of x, which is what bounds this form (12 TB/s out of the
+        // caches), but the CUs have to be covered.  Thirteen tokens, one / two / four tiles: 4096 x 8192 9.8 / 12.3 /
+        // 17.8 us, 8192 x 8192 16.5 / 13.7 / 19.2 us, 16384 x 16384 (sixteen tokens) 58 / 43 / 39 us.  Thirty-two
+        // 16-bit tokens go as two tiles of one workgroup: 8192 x 8192 18.1 us, as two workgroups 21.0.
+        constexpr int kMostTok = sizeof(T) == 2 ? 2 : 1;
+        if (kMostTok == 2 && batch > 16) {
+            if (M > 16 * cus) of_group(integral_constant<int, 2>{}, integral_constant<int, kMostTok>{});
+            else of_group(integral_constant<int, 1>{}, integral_constant<int, kMostTok>{});
+        } else if (M > 48 * cus) of_group(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+        else if (M > 16 * cus) of_group(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+        else of_group(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+        return launch_status();
     }
     auto go = [&](auto tb, auto rows) {
         constexpr int TB = decltype(tb)::value, kRows = decltype(rows)::value, kPieces = kRows < 4 ? 4 / kRows : 1;
