@@ -240,7 +240,7 @@ constexpr int kW4TileTokens = sizeof(T) == 2 ? 3 : 5;
 constexpr int kW4TileWaves = 8;
 constexpr int kW4Segment = 16;  // scales of a row that a wave keeps in LDS at a time
 template <class T>
-constexpr int kW4Exchange = kWave * 32 * static_cast<int>(sizeof(T)) / 4 / 2;  // 8 values of every lane: 1 or 2 KiB
+constexpr int kW4Exchange = kWave * 8 * static_cast<int>(sizeof(T));  // 8 values of every lane
 
 typedef f16 v8h __attribute__((ext_vector_type(8)));
 typedef bf16 v8b __attribute__((ext_vector_type(8)));
