@@ -143,48 +143,84 @@ __global__ __launch_bounds__(kSortMaxThreads) void expert_place_kernel(unsigned 
 
 // ---- rows to their places and back ------------------------------------------
 
-constexpr int kRowThreads = 256;
+constexpr int kRowWaves = 4;  // waves of a workgroup
 
-// out[pos[t][j]] = x[t], one workgroup per token and strip of kRowThreads vectors.
-template <class T, bool kDwords>
-__global__ __launch_bounds__(kRowThreads) void expert_gather_kernel(int tokens, int topk, int rows, int cols, const T* __restrict__ x,
+// A workgroup is one or more teams of `team_waves` waves, each with a token at a time: narrow rows leave no lanes idle.  A team
+// takes a strip of a vector per thread of a row.
+struct row_team {
+    int lane, wave, waves, first_wave, team, teams, threads, thread;
+    __device__ __forceinline__ explicit row_team(int team_waves) {
+        lane = threadIdx.x & (kWave - 1);
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+        waves = team_waves;
+        team = __builtin_amdgcn_readfirstlane(wave / team_waves);
+        teams = __builtin_amdgcn_readfirstlane(blockDim.x / kWave / team_waves);
+        first_wave = team * team_waves;
+        threads = team_waves * kWave;
+        thread = (wave - first_wave) * kWave + lane;
+    }
+};
+
+// A choice's row, or zeros where it has none: through a descriptor without a branch.
+template <class T, row_kind kKind>
+__device__ __forceinline__ void load_or_clear(row_values<T, 1, kKind>& v, const T* m, int64_t ld, int row, int rows, bool is) {
+    if constexpr (kKind == kOverlapRows) {
+        if (is) v.load(m, ld, row, rows);
+        else v.clear();
+    } else {
+        v.load(m, ld, is ? row : rows, rows);
+    }
+}
+
+// First column of a strip.  A strip that is cut short is a row of its own: it may be shorter than a vector, which kOverlapRows
+// cannot have, so there the last strip is moved back to end with the row instead.
+template <class T, row_kind kKind>
+__device__ __forceinline__ int strip_start(int strip, int width, int cols) {
+    const int first = strip * width;
+    return kKind == kOverlapRows ? max(0, min(first, cols - width)) : first;
+}
+
+// out[pos[t][j]] = x[t].
+template <class T, row_kind kKind>
+__global__ __launch_bounds__(kRowWaves * kWave) void expert_gather_kernel(int tokens, int topk, int rows, int cols, int team_waves, const T* __restrict__ x,
                                                                     int64_t ldx, const int* __restrict__ pos, T* __restrict__ out,
                                                                     int64_t ldout) {
-    const int first = blockIdx.y * kRowThreads * kVec<T>, here = min(cols - first, kRowThreads * kVec<T>);
-    for (int t = blockIdx.x; t < tokens; t += gridDim.x) {
-        row_values<T, 1, kDwords> v(threadIdx.x, kRowThreads);
-        v.load(x + t * ldx + first, here);
+    const row_team m(team_waves);
+    const int width = m.threads * kVec<T>, first = strip_start<T, kKind>(blockIdx.y, width, cols), here = min(cols - first, width);
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * m.teams + m.team; t < tokens; t += static_cast<int64_t>(gridDim.x) * m.teams) {
+        row_values<T, 1, kKind> v(m.thread, m.threads, here);
+        v.load(x + first, ldx, t, tokens);
         for (int j = 0; j < topk; ++j) {
-            const int p = pos[static_cast<int64_t>(t) * topk + j];
-            const bool is = p >= 0 && p < rows;
-            v.copy_to(out + (is ? p : 0) * ldout + first, is ? here : 0);
+            const int p = pos[t * topk + j];
+            if (p >= 0 && p < rows) v.store(out + first, ldout, p, rows);
         }
     }
 }
 
 // y[t] = sum_j w[t][j] xs[pos[t][j]], added in FP32 in the order of j; kBatch rows are on their way at a time.
-template <class T, bool kDwords>
-__global__ __launch_bounds__(kRowThreads) void expert_combine_kernel(int tokens, int topk, int rows, int cols, const T* __restrict__ xs,
+template <class T, row_kind kKind>
+__global__ __launch_bounds__(kRowWaves * kWave) void expert_combine_kernel(int tokens, int topk, int rows, int cols, int team_waves, const T* __restrict__ xs,
                                                                      int64_t ldxs, const int* __restrict__ pos,
                                                                      const float* __restrict__ weights, T* __restrict__ y, int64_t ldy) {
     constexpr int kBatch = 4;
-    const int first = blockIdx.y * kRowThreads * kVec<T>, here = min(cols - first, kRowThreads * kVec<T>);
-    for (int t = blockIdx.x; t < tokens; t += gridDim.x) {
+    const row_team m(team_waves);
+    const int width = m.threads * kVec<T>, first = strip_start<T, kKind>(blockIdx.y, width, cols), here = min(cols - first, width);
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * m.teams + m.team; t < tokens; t += static_cast<int64_t>(gridDim.x) * m.teams) {
         float acc[1][kVec<T>];
 #pragma unroll
         for (int i = 0; i < kVec<T>; ++i) acc[0][i] = 0.f;
-        row_values<T, 1, kDwords> sum(threadIdx.x, kRowThreads);
+        row_values<T, 1, kKind> sum(m.thread, m.threads, here);
         for (int j0 = 0; j0 < topk; j0 += kBatch) {
-            row_values<T, 1, kDwords> v[kBatch] = {sum, sum, sum, sum};
+            row_values<T, 1, kKind> v[kBatch] = {sum, sum, sum, sum};
             float w[kBatch];
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 const int j = min(j0 + b, topk - 1);
-                const int64_t s = static_cast<int64_t>(t) * topk + j;
+                const int64_t s = t * topk + j;
                 const int p = pos[s];
                 const bool is = j0 + b < topk && p >= 0 && p < rows;  // else zeros, which weigh nothing whatever the weight
                 w[b] = !is ? 0.f : weights != nullptr ? weights[s] : 1.f;
-                v[b].load(xs + (is ? p : 0) * ldxs + first, is ? here : 0);
+                load_or_clear(v[b], xs + first, ldxs, p, rows, is);
             }
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
@@ -194,76 +230,77 @@ __global__ __launch_bounds__(kRowThreads) void expert_combine_kernel(int tokens,
                 for (int i = 0; i < kVec<T>; ++i) acc[0][i] = __builtin_fmaf(w[b], f[0][i], acc[0][i]);
             }
         }
-        sum.store(y + t * ldy + first, here, acc);
+        sum.set(acc);
+        sum.store(y + first, ldy, t, tokens);
     }
 }
 
-// dxs[pos[t][j]] = w[t][j] dy[t],  dw[t][j] = <dy[t], xs[pos[t][j]]>: one workgroup per token; a choice's dot product is
+// dxs[pos[t][j]] = w[t][j] dy[t],  dw[t][j] = <dy[t], xs[pos[t][j]]>: a choice's dot product is
 // added over the thread's columns, the lanes and the waves in that fixed order.
-template <class T, bool kDwords>
-__global__ __launch_bounds__(kRowThreads) void expert_combine_grad_kernel(int tokens, int topk, int rows, int cols,
+template <class T, row_kind kKind>
+__global__ __launch_bounds__(kRowWaves * kWave) void expert_combine_grad_kernel(int tokens, int topk, int rows, int cols, int team_waves,
                                                                           const T* __restrict__ dy, int64_t lddy,
                                                                           const T* __restrict__ xs, int64_t ldxs,
                                                                           const int* __restrict__ pos, const float* __restrict__ weights,
                                                                           T* __restrict__ dxs, int64_t lddxs, float* __restrict__ dweights) {
-    constexpr int kWaves = kRowThreads / kWave, kBatch = 2;
-    constexpr int kStrip = kRowThreads * kVec<T>;
-    __shared__ float part[2][kBatch][kWaves];
-    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    constexpr int kBatch = 2;
+    __shared__ float part[2][kBatch][kRowWaves];
+    const row_team m(team_waves);
+    const int width = m.threads * kVec<T>;
     int turn = 0;
-    for (int t = blockIdx.x; t < tokens; t += gridDim.x)
+    // all teams walk as long as the first has tokens: the barrier is the workgroup's
+    for (int64_t lead = static_cast<int64_t>(blockIdx.x) * m.teams; lead < tokens; lead += static_cast<int64_t>(gridDim.x) * m.teams)
         for (int j0 = 0; j0 < topk; j0 += kBatch, turn ^= 1) {
+            const int64_t t = min(lead + m.team, static_cast<int64_t>(tokens) - 1);
+            const bool has_token = lead + m.team < tokens;
             int p[kBatch];
             float w[kBatch], dot[kBatch];
-            bool is[kBatch];
+            bool is[kBatch], any = false;
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
-                const int64_t s = static_cast<int64_t>(t) * topk + min(j0 + b, topk - 1);
+                const int64_t s = t * topk + min(j0 + b, topk - 1);
                 p[b] = pos[s];
-                is[b] = j0 + b < topk && p[b] >= 0 && p[b] < rows;
+                is[b] = has_token && j0 + b < topk && p[b] >= 0 && p[b] < rows;
                 w[b] = !is[b] ? 0.f : weights != nullptr ? weights[s] : 1.f;
                 dot[b] = 0.f;
+                any |= is[b];
             }
-            bool any = false;
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) any |= is[b];
             if (any)
-                for (int first = 0; first < cols; first += kStrip) {
-                    const int here = min(cols - first, kStrip);
-                    row_values<T, 1, kDwords> g(threadIdx.x, kRowThreads), v[kBatch] = {g, g};
-                    g.load(dy + t * lddy + first, here);
+                for (int strip = 0; strip * width < cols; ++strip) {
+                    const int first = strip_start<T, kKind>(strip, width, cols), here = min(cols - first, width);
+                    row_values<T, 1, kKind> g(m.thread, m.threads, here), v[kBatch] = {g, g};
+                    g.load(dy + first, lddy, t, tokens);
 #pragma unroll
-                    for (int b = 0; b < kBatch; ++b) {
-                        const bool read = is[b] && dweights != nullptr;
-                        v[b].load(xs + (read ? p[b] : 0) * ldxs + first, read ? here : 0);
-                    }
+                    for (int b = 0; b < kBatch; ++b) load_or_clear(v[b], xs + first, ldxs, p[b], rows, is[b] && dweights != nullptr);
                     float gf[1][kVec<T>];
                     g.get(gf);
 #pragma unroll
                     for (int b = 0; b < kBatch; ++b) {
-                        const bool write = is[b] && dxs != nullptr;
                         float f[1][kVec<T>];
                         v[b].get(f);
 #pragma unroll
                         for (int i = 0; i < kVec<T>; ++i) {
-                            dot[b] = __builtin_fmaf(gf[0][i], f[0][i], dot[b]);
+                            // columns of its own, and none that an earlier strip had
+                            const bool mine = kKind != kOverlapRows || (g.own(0, i) && first + g.column(0, i) >= strip * width);
+                            dot[b] = __builtin_fmaf(mine ? gf[0][i] : 0.f, mine ? f[0][i] : 0.f, dot[b]);
                             f[0][i] = gf[0][i] * w[b];
                         }
-                        g.store(dxs + (write ? p[b] : 0) * lddxs + first, write ? here : 0, f);
+                        v[b].set(f);
+                        if (is[b] && dxs != nullptr) v[b].store(dxs + first, lddxs, p[b], rows);
                     }
                 }
             if (dweights != nullptr) {
 #pragma unroll
                 for (int b = 0; b < kBatch; ++b) {
                     dot[b] = wave_allsum(dot[b]);
-                    if (lane == 0) part[turn][b][wave] = dot[b];
+                    if (m.lane == 0) part[turn][b][m.wave] = dot[b];
                 }
                 __syncthreads();
-                const int b = threadIdx.x;
-                if (b < kBatch && j0 + b < topk) {
-                    float sum = part[turn][b][0];
-                    for (int k = 1; k < kWaves; ++k) sum += part[turn][b][k];
-                    dweights[static_cast<int64_t>(t) * topk + j0 + b] = is[b] ? sum : 0.f;
+                const int b = m.thread;
+                if (b < kBatch && j0 + b < topk && has_token) {
+                    float sum = part[turn][b][m.first_wave];
+                    for (int k = 1; k < m.waves; ++k) sum += part[turn][b][m.first_wave + k];
+                    dweights[t * topk + j0 + b] = is[b] ? sum : 0.f;
                 }
             }
         }
@@ -290,18 +327,33 @@ bool choices_valid(int tokens, int topk) {
 }
 bool rows_valid(const void* p, int64_t ld, int cols, int type) { return p != nullptr && ld >= cols && aligned(p, type_bytes(type)); }
 
-// f(T*, kDwords) with the type of the rows and whether they can be read 16 bytes at a time
+// f(T*, kKind) with the type of the rows and how they are read
 template <class F>
-int with_rows(int type, bool dwords, F&& f) {
+int with_rows(int type, row_kind kind, F&& f) {
+    using std::integral_constant;
     return with_type(type, [&](auto* t) {
-        if constexpr (sizeof(*t) == 2)
-            if (!dwords) return f(t, std::false_type{});
-        return f(t, std::true_type{});
+        if constexpr (sizeof(*t) == 2) {
+            if (kind == kOverlapRows) return f(t, integral_constant<row_kind, kOverlapRows>{});
+            if (kind == kSingleRows) return f(t, integral_constant<row_kind, kSingleRows>{});
+        }
+        return f(t, integral_constant<row_kind, kDwordRows>{});
     });
 }
 
-// Workgroups over the tokens: one each up to a limit far above what the chip holds at a time.
-int token_grid(int tokens) { return std::min(tokens, 1 << 20); }
+// Waves to a token and the launch: a vector per thread up to four waves, several tokens to a workgroup below that.
+struct row_launch {
+    int team_waves, threads;
+    dim3 grid;
+};
+row_launch plan_rows(int tokens, int cols, int vec, bool strips) {
+    row_launch l;
+    l.team_waves = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(kRowWaves, ceil_div(cols, vec * kWave))));
+    const int teams = kRowWaves / l.team_waves;
+    l.threads = teams * l.team_waves * kWave;
+    // (a launch holds fewer than 2^32 threads; the teams walk on from there)
+    l.grid = dim3(static_cast<unsigned>(std::min<int64_t>(ceil_div(tokens, teams), 1 << 20)), strips ? static_cast<unsigned>(ceil_div(cols, vec * l.team_waves * kWave)) : 1u);
+    return l;
+}
 
 }  // namespace
 
@@ -348,11 +400,11 @@ extern "C" int hpcdnn_expert_gather(int type, int tokens, int topk, int rows, in
     if (!rows_valid(x, ldx, cols, type) || !rows_valid(out, ldout, cols, type) || pos == nullptr || !aligned(pos, 4))
         return HPCDNN_ERR_INVALID_VALUE;
     const size_t e = type_bytes(type);
-    return with_rows(type, rows_are_dwords(x, ldx, cols, e) && rows_are_dwords(out, ldout, cols, e), [&](auto* t, auto dwords) -> int {
+    return with_rows(type, kind_of(rows_are_dwords(x, ldx, cols, e) && rows_are_dwords(out, ldout, cols, e), cols), [&](auto* t, auto kind) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
-        const dim3 grid(token_grid(tokens), static_cast<unsigned>(ceil_div(cols, kRowThreads * kVec<T>)));
-        expert_gather_kernel<T, decltype(dwords)::value><<<grid, kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
-            tokens, topk, rows, cols, static_cast<const T*>(x), ldx, pos, static_cast<T*>(out), ldout);
+        const row_launch l = plan_rows(tokens, cols, kVec<T>, true);
+        expert_gather_kernel<T, decltype(kind)::value><<<l.grid, l.threads, 0, static_cast<hipStream_t>(stream)>>>(
+            tokens, topk, rows, cols, l.team_waves, static_cast<const T*>(x), ldx, pos, static_cast<T*>(out), ldout);
         return launch_status();
     });
 }
@@ -366,11 +418,11 @@ extern "C" int hpcdnn_expert_combine(int type, int tokens, int topk, int rows, i
         !aligned(weights, 4))
         return HPCDNN_ERR_INVALID_VALUE;
     const size_t e = type_bytes(type);
-    return with_rows(type, rows_are_dwords(xs, ldxs, cols, e) && rows_are_dwords(y, ldy, cols, e), [&](auto* t, auto dwords) -> int {
+    return with_rows(type, kind_of(rows_are_dwords(xs, ldxs, cols, e) && rows_are_dwords(y, ldy, cols, e), cols), [&](auto* t, auto kind) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
-        const dim3 grid(token_grid(tokens), static_cast<unsigned>(ceil_div(cols, kRowThreads * kVec<T>)));
-        expert_combine_kernel<T, decltype(dwords)::value><<<grid, kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
-            tokens, topk, rows, cols, static_cast<const T*>(xs), ldxs, pos, weights, static_cast<T*>(y), ldy);
+        const row_launch l = plan_rows(tokens, cols, kVec<T>, true);
+        expert_combine_kernel<T, decltype(kind)::value><<<l.grid, l.threads, 0, static_cast<hipStream_t>(stream)>>>(
+            tokens, topk, rows, cols, l.team_waves, static_cast<const T*>(xs), ldxs, pos, weights, static_cast<T*>(y), ldy);
         return launch_status();
     });
 }
@@ -388,10 +440,11 @@ extern "C" int hpcdnn_expert_combine_grad(int type, int tokens, int topk, int ro
     const size_t e = type_bytes(type);
     const bool all_dwords = rows_are_dwords(dy, lddy, cols, e) && (dweights == nullptr || rows_are_dwords(xs, ldxs, cols, e)) &&
                             (dxs == nullptr || rows_are_dwords(dxs, lddxs, cols, e));
-    return with_rows(type, all_dwords, [&](auto* t, auto dwords) -> int {
+    return with_rows(type, kind_of(all_dwords, cols), [&](auto* t, auto kind) -> int {
         using T = std::remove_pointer_t<decltype(t)>;
-        expert_combine_grad_kernel<T, decltype(dwords)::value><<<token_grid(tokens), kRowThreads, 0, static_cast<hipStream_t>(stream)>>>(
-            tokens, topk, rows, cols, static_cast<const T*>(dy), lddy, static_cast<const T*>(xs), ldxs, pos, weights,
+        const row_launch l = plan_rows(tokens, cols, kVec<T>, false);
+        expert_combine_grad_kernel<T, decltype(kind)::value><<<l.grid, l.threads, 0, static_cast<hipStream_t>(stream)>>>(
+            tokens, topk, rows, cols, l.team_waves, static_cast<const T*>(dy), lddy, static_cast<const T*>(xs), ldxs, pos, weights,
             static_cast<T*>(dxs), lddxs, dweights);
         return launch_status();
     });

@@ -15,14 +15,18 @@ constexpr int kNormRowWaves = 4;     // rows per workgroup where a wave takes a 
 constexpr int kNormMaxWaves = 16;
 
 // Parameters of the thread's columns in FP32; `fill` where there are none (and behind the last column).
-template <class T, class W, int NV, bool kDwords>
-__device__ __forceinline__ void load_params(const W* p, float fill, const row_values<T, NV, kDwords>& s, int cols, float (&out)[NV][kVec<T>]) {
+template <class T, class W, int NV, row_kind kKind>
+__device__ __forceinline__ void load_params(const W* p, float fill, const row_values<T, NV, kKind>& s, int cols, float (&out)[NV][kVec<T>]) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
 #pragma unroll
         for (int i = 0; i < kVec<T>; ++i) out[v][i] = fill;
         if (p == nullptr) continue;
-        if constexpr (kDwords) {
+        if constexpr (kKind == kSingleRows) {
+#pragma unroll
+            for (int i = 0; i < kVec<T>; ++i)
+                if (s.own(v, i)) out[v][i] = static_cast<float>(p[s.column(v, i)]);
+        } else {
 #pragma unroll
             for (int i = 0; i < kVec<T>; i += kVec<W>) {
                 if (s.column(v, i) >= cols) continue;
@@ -31,10 +35,6 @@ __device__ __forceinline__ void load_params(const W* p, float fill, const row_va
 #pragma unroll
                 for (int k = 0; k < kVec<W>; ++k) out[v][i + k] = f[k];
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kVec<T>; ++i)
-                if (s.column(v, i) < cols) out[v][i] = static_cast<float>(p[s.column(v, i)]);
         }
     }
 }
@@ -44,7 +44,7 @@ __device__ __forceinline__ void load_params(const W* p, float fill, const row_va
 //   mu = sum n_w mu_w / C,   M2 = sum M2_w + n_w (mu_w - mu)^2,
 // so nothing cancels (sum x^2 - C mu^2 would lose the variance of rows with a large mean) and a row costs one barrier.
 // The next row is loaded into the registers of the present one as soon as that is unpacked.
-template <class T, class W, int NV, bool kWaveRow, bool kDwords>
+template <class T, class W, int NV, bool kWaveRow, row_kind kKind>
 __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer_norm_kernel(
     int64_t rows, int cols, const T* __restrict__ x, int64_t ldx, const W* __restrict__ w, const W* __restrict__ b, float eps,
     T* __restrict__ y, int64_t ldy, float* __restrict__ mean, float* __restrict__ rstd) {
@@ -55,17 +55,17 @@ __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer
     const int64_t step = kWaveRow ? static_cast<int64_t>(gridDim.x) * kNormRowWaves : gridDim.x;
     int64_t r = kWaveRow ? static_cast<int64_t>(blockIdx.x) * kNormRowWaves + wave : blockIdx.x;
     if (r >= rows) return;
-    row_values<T, NV, kDwords> cur(kWaveRow ? lane : threadIdx.x, kWaveRow ? kWave : blockDim.x);
-    auto load = [&](int64_t row) { cur.load(x + (row < rows ? row : 0) * ldx, row < rows ? cols : 0); };
-    load(r);
+    row_values<T, NV, kKind> cur(kWaveRow ? lane : threadIdx.x, kWaveRow ? kWave : blockDim.x, cols);
+    cur.load(x, ldx, r, rows);
+    loads_start_here();
     float wf[NV][kVec<T>], bf[NV][kVec<T>];
-    load_params<T, W, NV, kDwords>(w, 1.f, cur, cols, wf);
-    load_params<T, W, NV, kDwords>(b, 0.f, cur, cols, bf);
+    load_params<T, W, NV, kKind>(w, 1.f, cur, cols, wf);
+    load_params<T, W, NV, kKind>(b, 0.f, cur, cols, bf);
     int valid = 0;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int i = 0; i < kVec<T>; ++i) valid += cur.column(v, i) < cols;
+        for (int i = 0; i < kVec<T>; ++i) valid += cur.own(v, i);
     const float n_wave = wave_allsum(static_cast<float>(valid));
     const float n_cols = static_cast<float>(cols);
     // columns of wave (lane & 15): what the join below weighs that wave's mean with
@@ -79,18 +79,19 @@ __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer
     for (int turn = 0; r < rows; r += step, turn ^= 1) {
         float f[NV][kVec<T>], sum = 0.f;
         cur.get(f);
-        load(r + step);
+        cur.load(x, ldx, r + step, rows);
+        loads_start_here();
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int i = 0; i < kVec<T>; ++i) sum += f[v][i];
+            for (int i = 0; i < kVec<T>; ++i) sum += kKind != kOverlapRows || cur.own(v, i) ? f[v][i] : 0.f;  // (zeros behind the end)
         // divided, not multiplied by a reciprocal: a row of equal values then has exactly that mean, and no spread
         float mu = wave_allsum(sum) / fmaxf(n_wave, 1.f), m2 = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) {
-                const float d = cur.column(v, i) < cols ? f[v][i] - mu : 0.f;
+                const float d = cur.own(v, i) ? f[v][i] - mu : 0.f;
                 m2 = __builtin_fmaf(d, d, m2);
             }
         m2 = wave_allsum(m2);
@@ -110,7 +111,9 @@ __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) f[v][i] = __builtin_fmaf((f[v][i] - mu) * rs, wf[v][i], bf[v][i]);
-        cur.store(y + r * ldy, cols, f);
+        row_values<T, NV, kKind> out(cur.t, cur.n, cols);
+        out.set(f);
+        out.store(y, ldy, r, rows);
         if ((kWaveRow ? lane : static_cast<int>(threadIdx.x)) == 0) {
             if (mean != nullptr) mean[r] = mu;
             if (rstd != nullptr) rstd[r] = rs;
@@ -123,7 +126,7 @@ __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer
 // their order at the end, and the workgroup writes one partial row of each, [workgroup][2][cols] in the workspace, added in
 // the workgroups' order by layer_norm_params_kernel.  So dw and db do not depend on timing, and with sixteen waves to a
 // workgroup the partial rows stay few: they are the only traffic beside x, dy and dx.
-template <class T, class W, int NV, bool kWaveRow, bool kDwords>
+template <class T, class W, int NV, bool kWaveRow, row_kind kKind>
 __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(
     int64_t rows, int cols, int row_waves, const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x, int64_t ldx,
     const W* __restrict__ w, const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx, int64_t lddx,
@@ -138,25 +141,26 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(
     const int64_t step = static_cast<int64_t>(gridDim.x) * teams;
     const int64_t block_row = static_cast<int64_t>(blockIdx.x) * teams;
     int64_t r = block_row + team;
-    row_values<T, NV, kDwords> cx((wave - first_wave) * kWave + lane, row_waves * kWave), cd(cx.t, cx.n);
+    row_values<T, NV, kKind> cx((wave - first_wave) * kWave + lane, row_waves * kWave, cols), cd(cx.t, cx.n, cols);
     const float inv_cols = 1.f / static_cast<float>(cols);
     constexpr bool kKeep = NV * kVec<T> <= 8;  // w in registers; wider rows read it again (from L2), or they would spill
     float wf[NV][kVec<T>], dw[NV][kVec<T>], db[NV][kVec<T>];
-    if (kKeep) load_params<T, W, NV, kDwords>(w, 1.f, cx, cols, wf);
+    if (kKeep) load_params<T, W, NV, kKind>(w, 1.f, cx, cols, wf);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int i = 0; i < kVec<T>; ++i) dw[v][i] = db[v][i] = 0.f;
     float next_mu, next_rs;
-    // Behind the last row: zeros, which add nothing.  The statistics come as vector loads too: a scalar load in flight
-    // would be waited for with the LDS accesses of the exchange between the waves, which share its counter.
+    // The statistics come as vector loads too: a scalar load in flight would be waited for with the LDS accesses of the
+    // exchange between the waves, which share its counter.
     auto load = [&](int64_t row) {
         const bool is = row < rows;
-        const int64_t at = is ? row : 0;
-        cx.load(x + at * ldx, is ? cols : 0);
-        cd.load(dy + at * lddy, is ? cols : 0);
-        next_mu = buffer_load_f(make_rsrc(mean + at, is ? 4 : 0), 0);
-        next_rs = buffer_load_f(make_rsrc(rstd + at, is ? 4 : 0), 0);
+        cx.load(x, ldx, row, rows);
+        cd.load(dy, lddy, row, rows);
+        const int64_t at = is ? row : rows - 1;
+        next_mu = buffer_load_f(make_rsrc(mean + at, kKind == kOverlapRows || is ? 4 : 0), 0);
+        next_rs = buffer_load_f(make_rsrc(rstd + at, kKind == kOverlapRows || is ? 4 : 0), 0);
+        loads_start_here();
     };
     load(r);
     int turn = 0;
@@ -168,18 +172,22 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(
         float xh[NV][kVec<T>], g[NV][kVec<T>];
         cx.get(xh);
         cd.get(g);
-        if (!kKeep) load_params<T, W, NV, kDwords>(w, 1.f, cx, cols, wf);
+        if (!kKeep) load_params<T, W, NV, kKind>(w, 1.f, cx, cols, wf);
         load(r + step);
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) {
                 xh[v][i] = (xh[v][i] - mu) * rs;
-                dw[v][i] = __builtin_fmaf(g[v][i], xh[v][i], dw[v][i]);
-                db[v][i] += g[v][i];
+                // A team without a row in the last turn must add nothing: it has zeros, or else (kOverlapRows) the last row.
+                if (kKind != kOverlapRows || r < rows) {
+                    dw[v][i] = __builtin_fmaf(g[v][i], xh[v][i], dw[v][i]);
+                    db[v][i] += g[v][i];
+                }
                 g[v][i] *= wf[v][i];
-                g_sum += g[v][i];
-                gx_sum = __builtin_fmaf(g[v][i], xh[v][i], gx_sum);
+                const float term = kKind != kOverlapRows || cx.own(v, i) ? g[v][i] : 0.f;
+                g_sum += term;
+                gx_sum = __builtin_fmaf(term, xh[v][i], gx_sum);
             }
         g_sum = wave_allsum(g_sum);
         gx_sum = wave_allsum(gx_sum);
@@ -194,12 +202,13 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(
             gx_sum = row16_allsum(has ? part[turn][1][first_wave + (lane & 15)] : 0.f);
         }
         const float a = g_sum * inv_cols, c = gx_sum * inv_cols;
-        const bool is = r < rows && dx != nullptr;  // else dropped
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) g[v][i] = rs * (g[v][i] - a - xh[v][i] * c);
-        cx.store(dx + (is ? r : 0) * lddx, is ? cols : 0, g);
+        row_values<T, NV, kKind> out(cx.t, cx.n, cols);
+        out.set(g);
+        if (kKind != kOverlapRows || dx != nullptr) out.store(dx, lddx, r, dx != nullptr ? rows : 0);
     }
     if (partial == nullptr) return;
     float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * cols;
@@ -209,7 +218,7 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) {
                 const int c = cx.column(v, i);
-                if (c < cols) {
+                if (cx.own(v, i)) {
                     out[c] = dw[v][i];
                     out[cols + c] = db[v][i];
                 }
@@ -235,9 +244,10 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(
     }
     for (int c = threadIdx.x; c < cols; c += blockDim.x) {
         int value = c / n, thread = c - value * n;
-        if (kDwords) {
+        if (kKind != kSingleRows) {
             const int vec = c / kVec<T>, v = vec / n;
-            value = v * kVec<T> + c % kVec<T>;
+            const int at = kKind == kOverlapRows ? min(vec * kVec<T>, cols - kVec<T>) : vec * kVec<T>;
+            value = v * kVec<T> + c - at;
             thread = vec - v * n;
         }
         const float* a = joined + value * pitch + thread;
@@ -298,15 +308,17 @@ norm_shape shape_of(int cols, int vec) {
 // CU measured 2 % faster for 30000 x 512 BF16, but 5 to 11 % slower from 2048 columns on: the partial rows double.)
 int grad_blocks(int rows) { return std::min(rows, device_cus()); }
 
-// f(NV, kWaveRow, kDwords) as compile-time constants
+// f(NV, kWaveRow, kKind) as compile-time constants
 template <class T, class F>
-void with_shape(const norm_shape& s, bool dwords, F&& f) {
+void with_shape(const norm_shape& s, row_kind kind, F&& f) {
     using std::integral_constant;
     auto more = [&](auto nv, auto wave_row) {
-        if constexpr (sizeof(T) == 4) f(nv, wave_row, std::true_type{});
-        else if (dwords) f(nv, wave_row, std::true_type{});
-        else f(nv, wave_row, std::false_type{});
+        if constexpr (sizeof(T) == 2)
+            if (kind != kDwordRows) return f(nv, wave_row, integral_constant<row_kind, kOverlapRows>{});
+        f(nv, wave_row, integral_constant<row_kind, kDwordRows>{});
     };
+    if constexpr (sizeof(T) == 2)
+        if (kind == kSingleRows) return f(integral_constant<int, 1>{}, std::true_type{}, integral_constant<row_kind, kSingleRows>{});
     if (s.wave_row) {
         if (s.nv == 1) more(integral_constant<int, 1>{}, std::true_type{});
         else more(integral_constant<int, 2>{}, std::true_type{});
@@ -322,8 +334,9 @@ int launch_norm(int rows, int cols, const void* x, int64_t ldx, const void* w, c
     const int64_t blocks = s.wave_row ? ceil_div(rows, kNormRowWaves) : rows;
     const int64_t most = static_cast<int64_t>(device_cus()) * (2048 / s.threads);
     const int grid = static_cast<int>(blocks < most ? blocks : most);
-    with_shape<T>(s, rows_are_dwords(x, ldx, cols, sizeof(T)) && rows_are_dwords(y, ldy, cols, sizeof(T)), [&](auto nv, auto wave_row, auto dwords) {
-        layer_norm_kernel<T, W, decltype(nv)::value, decltype(wave_row)::value, decltype(dwords)::value><<<grid, s.threads, 0, stream>>>(
+    const row_kind kind = kind_of(rows_are_dwords(x, ldx, cols, sizeof(T)) && rows_are_dwords(y, ldy, cols, sizeof(T)), cols);
+    with_shape<T>(s, kind, [&](auto nv, auto wave_row, auto rows_kind) {
+        layer_norm_kernel<T, W, decltype(nv)::value, decltype(wave_row)::value, decltype(rows_kind)::value><<<grid, s.threads, 0, stream>>>(
             rows, cols, static_cast<const T*>(x), ldx, static_cast<const W*>(w), static_cast<const W*>(b), eps, static_cast<T*>(y), ldy,
             mean, rstd);
     });
@@ -341,8 +354,8 @@ int launch_grad(int rows, int cols, const void* dy, int64_t lddy, const void* x,
         const size_t lds = teams > 1 && partial ? 2 * sizeof(float) * s.nv * kVec<T> * (row_waves * kWave + 8) : 0;
         const bool all_dwords = rows_are_dwords(x, ldx, cols, sizeof(T)) && rows_are_dwords(dy, lddy, cols, sizeof(T)) &&
                                 (dx == nullptr || rows_are_dwords(dx, lddx, cols, sizeof(T)));
-        with_shape<T>(s, all_dwords, [&](auto nv, auto wave_row, auto dwords) {
-            layer_norm_grad_kernel<T, W, decltype(nv)::value, decltype(wave_row)::value, decltype(dwords)::value>
+        with_shape<T>(s, kind_of(all_dwords, cols), [&](auto nv, auto wave_row, auto rows_kind) {
+            layer_norm_grad_kernel<T, W, decltype(nv)::value, decltype(wave_row)::value, decltype(rows_kind)::value>
                 <<<grid, teams * row_waves * kWave, lds, stream>>>(
                     rows, cols, row_waves, static_cast<const T*>(dy), lddy, static_cast<const T*>(x), ldx, static_cast<const W*>(w), mean,
                     rstd, static_cast<T*>(dx), lddx, partial);

@@ -61,11 +61,6 @@ __device__ __forceinline__ v4u load_row(const T* row, int col, int cols) {
     return v4u{0u, 0u, 0u, 0u};
 }
 
-// Whether rows of this matrix are whole dwords (host).
-inline bool rows_are_dwords(const void* p, int64_t ld, int cols, size_t elem) {
-    return reinterpret_cast<uintptr_t>(p) % 4 == 0 && (ld * static_cast<int64_t>(elem)) % 4 == 0 && (cols * elem) % 4 == 0;
-}
-
 template <class T>
 __device__ __forceinline__ void unpack(v4u u, float (&f)[kVec<T>]) {
     if constexpr (std::is_same_v<T, float>) {
@@ -135,57 +130,106 @@ struct row_buffer {
     }
 };
 
-// The values of a row that one thread of the `n` that share it holds, NV vectors of kVec.  kDwords: consecutive values, 16
-// bytes at a time, vector v from column (v n + t) kVec on.  Else (16-bit rows that start at odd addresses or hold an odd
-// number of values) single ones, n apart, so that the threads of a wave still touch consecutive addresses.
-template <class T, int NV, bool kDwords>
+// How the threads that share a row hold its values, NV vectors of kVec each.
+//  kDwordRows   rows on 4-byte addresses that hold whole dwords: vector v of thread t is columns (v n + t) kVec ..., through a
+//               descriptor that ends it.
+//  kOverlapRows any other row of at least kVec values (16-bit rows of odd length, or at odd addresses): the same vectors from
+//               any address, and those that would pass the end of the row are moved back to end with it.  What such a vector
+//               shares with its neighbour is not its own: left out of every sum, and stored twice with the same value.  So
+//               there is no branch here either.
+//  kSingleRows  shorter ones, value by value through the descriptor.
+enum row_kind { kDwordRows, kOverlapRows, kSingleRows };
+
+template <class T, int NV, row_kind kKind>
 struct row_values {
-    static_assert(kDwords || sizeof(T) == 2, "FP32 rows are whole dwords");
-    int t, n;
-    v4u u[kDwords ? NV : 1];
-    T single[kDwords ? 1 : NV * kVec<T>];
-    __device__ __forceinline__ row_values(int thread, int threads) : t(thread), n(threads) {}
-    __device__ __forceinline__ int column(int v, int i) const { return kDwords ? (v * n + t) * kVec<T> + i : (v * kVec<T> + i) * n + t; }
-    __device__ __forceinline__ void load(const T* row, int cols) {
-        const row_buffer<T, kDwords> b(row, cols);
-        if constexpr (kDwords) {
+    static_assert(kKind == kDwordRows || sizeof(T) == 2, "FP32 rows are whole dwords");
+    int t, n, cols;
+    v4u u[kKind == kSingleRows ? 1 : NV];
+    T single[kKind == kSingleRows ? NV * kVec<T> : 1];
+    __device__ __forceinline__ row_values(int thread, int threads, int columns) : t(thread), n(threads), cols(columns) {}
+    __device__ __forceinline__ int first_own(int v) const { return (v * n + t) * kVec<T>; }
+    __device__ __forceinline__ int column(int v, int i) const {
+        if constexpr (kKind == kSingleRows) return (v * kVec<T> + i) * n + t;
+        else if constexpr (kKind == kOverlapRows) return min(first_own(v), cols - kVec<T>) + i;
+        else return first_own(v) + i;
+    }
+    __device__ __forceinline__ bool own(int v, int i) const {
+        return kKind == kOverlapRows ? column(v, i) >= first_own(v) : column(v, i) < cols;
+    }
+    // Row `row` of the matrix at m.  Behind its last row: zeros (kOverlapRows: the last row).
+    __device__ __forceinline__ void load(const T* m, int64_t ld, int64_t row, int64_t rows) {
+        const bool is = row < rows;
+        if constexpr (kKind == kOverlapRows) {
+            const T* r = m + (is ? row : rows - 1) * ld;
 #pragma unroll
-            for (int v = 0; v < NV; ++v) u[v] = b.load16(column(v, 0));
+            for (int v = 0; v < NV; ++v) u[v] = load16(r + column(v, 0));
+        } else {
+            const row_buffer<T, kKind == kDwordRows> b(m + (is ? row : 0) * ld, is ? cols : 0);
+            if constexpr (kKind == kDwordRows) {
+#pragma unroll
+                for (int v = 0; v < NV; ++v) u[v] = b.load16(column(v, 0));
+            } else {
+#pragma unroll
+                for (int k = 0; k < NV * kVec<T>; ++k) single[k] = b.load1(k * n + t);
+            }
+        }
+    }
+    __device__ __forceinline__ void clear() {
+        if constexpr (kKind == kSingleRows) {
+#pragma unroll
+            for (int k = 0; k < NV * kVec<T>; ++k) single[k] = static_cast<T>(0.f);
         } else {
 #pragma unroll
-            for (int k = 0; k < NV * kVec<T>; ++k) single[k] = b.load1(k * n + t);
+            for (int v = 0; v < NV; ++v) u[v] = v4u{0u, 0u, 0u, 0u};
         }
     }
     __device__ __forceinline__ void get(float (&f)[NV][kVec<T>]) const {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if constexpr (kDwords) unpack<T>(u[v], f[v]);
-            else
+            if constexpr (kKind == kSingleRows) {
 #pragma unroll
                 for (int i = 0; i < kVec<T>; ++i) f[v][i] = static_cast<float>(single[v * kVec<T> + i]);
+            } else {
+                unpack<T>(u[v], f[v]);
+            }
         }
     }
-    __device__ __forceinline__ void copy_to(T* row, int cols) const {
-        const row_buffer<T, kDwords> b(row, cols);
-        if constexpr (kDwords) {
-#pragma unroll
-            for (int v = 0; v < NV; ++v) b.store16_once(column(v, 0), u[v]);
-        } else {
-#pragma unroll
-            for (int k = 0; k < NV * kVec<T>; ++k) b.store1(k * n + t, single[k]);
-        }
-    }
-    __device__ __forceinline__ void store(T* row, int cols, const float (&f)[NV][kVec<T>]) const {
-        const row_buffer<T, kDwords> b(row, cols);
+    __device__ __forceinline__ void set(const float (&f)[NV][kVec<T>]) {
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            if constexpr (kDwords) b.store16_once(column(v, 0), pack<T>(f[v]));
-            else
+            if constexpr (kKind == kSingleRows) {
 #pragma unroll
-                for (int i = 0; i < kVec<T>; ++i) b.store1(column(v, i), static_cast<T>(f[v][i]));
+                for (int i = 0; i < kVec<T>; ++i) single[v * kVec<T> + i] = static_cast<T>(f[v][i]);
+            } else {
+                u[v] = pack<T>(f[v]);
+            }
+        }
+    }
+    // Behind the last row: dropped (kOverlapRows: to the last row, whose values they are).
+    __device__ __forceinline__ void store(T* m, int64_t ld, int64_t row, int64_t rows) const {
+        const bool is = row < rows;
+        if constexpr (kKind == kOverlapRows) {
+            T* r = m + (is ? row : rows - 1) * ld;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) __builtin_nontemporal_store(u[v], reinterpret_cast<v4u_any*>(r + column(v, 0)));
+        } else {
+            const row_buffer<T, kKind == kDwordRows> b(m + (is ? row : 0) * ld, is ? cols : 0);
+            if constexpr (kKind == kDwordRows) {
+#pragma unroll
+                for (int v = 0; v < NV; ++v) b.store16_once(column(v, 0), u[v]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < NV * kVec<T>; ++k) b.store1(k * n + t, single[k]);
+            }
         }
     }
 };
+
+// Host: whether rows of this matrix are whole dwords, and the kind of a call all of whose matrices are (or are not).
+inline bool rows_are_dwords(const void* p, int64_t ld, int cols, size_t elem) {
+    return reinterpret_cast<uintptr_t>(p) % 4 == 0 && (ld * static_cast<int64_t>(elem)) % 4 == 0 && (cols * elem) % 4 == 0;
+}
+inline row_kind kind_of(bool all_dwords, int cols) { return all_dwords ? kDwordRows : cols >= kVec<f16> ? kOverlapRows : kSingleRows; }
 
 // Put behind loads whose values are for the next turn of a loop: memory might have changed, as far as the compiler knows, so
 // it cannot move them (as it does with plain loads) to where that turn uses them, and they stay in flight over this one.

@@ -608,7 +608,7 @@ extern "C" int hpcdnn_w4_gemv(int type, int batch, int M, int N, int group, floa
                               int64_t ldy, void* stream) {
     using namespace hpcdnn;
     const int shift = shift_of(group);
-    if (!type_valid(type) || batch < 0 || M < 0 || N < 0 || shift < 0 || N > HPCDNN_W4_MAX_COLS || batch > HPCDNN_W4_MAX_BATCH)
+    if (!type_valid(type) || batch < 0 || M < 0 || N < 0 || shift < 0 || N > HPCDNN_W4_MAX_COLS || M > HPCDNN_W4_MAX_ROWS || batch > HPCDNN_W4_MAX_BATCH)
         return HPCDNN_ERR_INVALID_VALUE;
     if (batch == 0 || M == 0) return HPCDNN_OK;
     const size_t e = type_bytes(type);

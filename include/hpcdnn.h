@@ -490,9 +490,10 @@ int hpcdnn_layer_norm_grad(int type, int wtype, int rows, int cols, const void* 
  * column in the low half; `ldq` is its length in bytes, a multiple of 4, and q is 4-byte aligned.  `scales`
  * (of `type`) and `zeros` (bytes, 0 .. 15; NULL: 8 everywhere) hold ceil(N / group) values per row with row
  * length `ldg`; group is 32, 64 or 128.  beta == 0 never reads y.  What stands behind column N in the last
- * byte and group is not used.  batch <= HPCDNN_W4_MAX_BATCH, N <= HPCDNN_W4_MAX_COLS.  The weights enter
+ * byte and group is not used.  batch <= HPCDNN_W4_MAX_BATCH, M <= HPCDNN_W4_MAX_ROWS, N <= HPCDNN_W4_MAX_COLS.  The weights enter
  * exactly, but x must stay a factor of 64 below the largest FP32 number, and an infinity in x gives infinities or NaN. */
 #define HPCDNN_W4_MAX_BATCH 65536
+#define HPCDNN_W4_MAX_ROWS (1 << 30)
 #define HPCDNN_W4_MAX_COLS (1 << 24)
 int hpcdnn_w4_gemv(int type, int batch, int M, int N, int group, float alpha, const uint8_t* q, int64_t ldq, const void* scales,
                    const uint8_t* zeros, int64_t ldg, const void* x, int64_t ldx, float beta, void* y, int64_t ldy, void* stream);

@@ -64,7 +64,7 @@ def _w4(L, type_=1, batch=2, M=4, N=40, group=32, q=P, ldq=20, s=P, z=P, ldg=2, 
     return L.hpcdnn_w4_gemv(type_, batch, M, N, group, 1.0, q, ldq, s, z, ldg, x, ldx, 0.0, y, ldy, None)
 
 
-@pytest.mark.parametrize("bad", [dict(type_=3), dict(batch=-1), dict(batch=65537), dict(M=-1), dict(N=-1), dict(N=(1 << 24) + 1), dict(group=16),
+@pytest.mark.parametrize("bad", [dict(type_=3), dict(batch=-1), dict(batch=65537), dict(M=-1), dict(M=(1 << 30) + 1, ldy=(1 << 30) + 1), dict(N=-1), dict(N=(1 << 24) + 1), dict(group=16),
                                  dict(group=48), dict(group=256), dict(q=None), dict(q=C.c_void_p(0x1002)), dict(ldq=16), dict(ldq=22),
                                  dict(s=None), dict(s=ODD), dict(ldg=1), dict(x=None), dict(x=ODD), dict(ldx=39), dict(y=None), dict(ldy=3)])
 def test_w4_gemv_refuses(L, bad):
