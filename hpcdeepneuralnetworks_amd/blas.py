@@ -390,9 +390,7 @@ def _type(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _on_device(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int) -> None:
-    if isinstance(t, torch.Tensor) and t.dtype == dtype and t.get_device() == dev:
-        return
+def _refuse(t, name: str, dtype: torch.dtype) -> None:
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype):
         raise HpcdnnError(f"{name} must be a {dtype} tensor on the GPU")
     raise HpcdnnError(f"{name} is on {t.device}, which is not the current device")
@@ -400,21 +398,25 @@ def _on_device(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int) -> None
 
 def _rows(t: torch.Tensor, rows: int, cols: int, name: str, dtype: torch.dtype, dev: int):
     """Pointer and row stride of a 2-D tensor with contiguous columns."""
-    _on_device(t, name, dtype, dev)
-    shape = t.shape
-    if len(shape) != 2 or shape[0] < rows or shape[1] < cols:
-        raise HpcdnnError(f"{name} must be 2-D with at least {rows}x{cols} elements, got {tuple(shape)}")
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev:
+        _refuse(t, name, dtype)
     stride = t.stride()
-    if stride[1] != 1 and shape[1] > 1:
+    if len(stride) != 2:
+        raise HpcdnnError(f"{name} must be 2-D with at least {rows}x{cols} elements, got {tuple(t.shape)}")
+    have, width = t.shape
+    if have < rows or width < cols:
+        raise HpcdnnError(f"{name} must be 2-D with at least {rows}x{cols} elements, got {tuple(t.shape)}")
+    if stride[1] != 1 and width > 1:
         raise HpcdnnError(f"{name} must have contiguous columns")
-    return t.data_ptr(), stride[0] if shape[0] > 1 else max(shape[1], 1)
+    return t.data_ptr(), stride[0] if have > 1 else max(width, 1)
 
 
 def _flat(t: torch.Tensor | None, n: int, name: str, dtype: torch.dtype, dev: int):
     """Pointer of a contiguous tensor of at least n elements, None for None."""
     if t is None:
         return None
-    _on_device(t, name, dtype, dev)
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev:
+        _refuse(t, name, dtype)
     if t.numel() < n or not t.is_contiguous():
         raise HpcdnnError(f"{name} must be contiguous with at least {n} elements")
     return t.data_ptr()
@@ -429,12 +431,13 @@ def _scratch(ws: torch.Tensor | None, dev: int):
 
 
 def _param_type(params, dtype: torch.dtype) -> torch.dtype:
+    """The one type of those parameters that are given."""
     kind = None
     for p in params:
         if p is not None:
             if kind is None:
                 kind = p.dtype
-            if p.dtype != kind or (kind != torch.float32 and kind != dtype):
+            if p.dtype is not kind or (kind is not torch.float32 and kind is not dtype):
                 raise HpcdnnError("w, b and their gradients must share one type: float32 or that of the rows")
     return torch.float32 if kind is None else kind
 
