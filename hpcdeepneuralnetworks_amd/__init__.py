@@ -1,4 +1,5 @@
-"""hpcdnn for AMD MI355X: FP32 SGEMM, ABFT-SGEMM, SAXPY and SDOT as hand-written gfx950 HIP kernels.
+"""hpcdnn for AMD MI355X: FP32 SGEMM, ABFT-SGEMM, SAXPY and SDOT and the operators of a transformer layer around its products
+(layer norm, 4-bit products, expert reordering) as hand-written gfx950 HIP kernels.
 
 ``blas`` mirrors the reference's kernel entry points on torch device tensors;
 ``_lib`` is the raw ctypes binding of the C ABI (``include/hpcdnn.h``).

@@ -1,5 +1,6 @@
 /*
- * hpcdnn -- FP32 BLAS level-1/3 + ABFT-SGEMM for AMD MI355X (gfx950).
+ * hpcdnn -- FP32 BLAS level-1/3 + ABFT-SGEMM for AMD MI355X (gfx950), and the
+ * operators of a transformer layer around its products (FP32, FP16, BF16).
  *
  * C ABI of libhpcdnn.so.  Plain pointers and sizes only; every device pointer
  * is memory the caller allocated on the current HIP device, every `stream` is
@@ -52,7 +53,7 @@ extern "C" {
 #define HPCDNN_OP_OFFLINE_FT_SGEMM 4
 #define HPCDNN_OP_FT_SGEMM_CM_NT 5     /* M, N, K as passed to hpcdnn_ft_sgemm_cm_nt */
 #define HPCDNN_OP_LAYER_NORM_GRAD 6    /* M = rows, N = cols */
-#define HPCDNN_OP_EXPERT_SORT 7        /* M = tokens, N = topk, K = experts */
+#define HPCDNN_OP_EXPERT_SORT 7        /* M = tokens, N = topk, K = experts; 0 bytes where none is needed */
 
 /* Element types of the layer operators (everything above them is FP32). */
 #define HPCDNN_F32 0
