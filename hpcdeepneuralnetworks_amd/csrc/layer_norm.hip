@@ -213,15 +213,15 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(
     if (partial == nullptr) return;
     float* out = partial + static_cast<int64_t>(blockIdx.x) * 2 * cols;
     if (teams == 1) {
+        // 16 bytes at a time (value by value, 392 x 15808 BF16 took 35.4 us instead of 21.5); what vectors share at the end of
+        // a row (kOverlapRows) is stored twice with the same value here too
+        const row_buffer<float, true> to_w(out, cols), to_b(out + cols, cols);
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int i = 0; i < kVec<T>; ++i) {
-                const int c = cx.column(v, i);
-                if (cx.own(v, i)) {
-                    out[c] = dw[v][i];
-                    out[cols + c] = db[v][i];
-                }
+            for (int i = 0; i < kVec<T>; i += 4) {
+                to_w.store16(cx.column(v, i), __builtin_bit_cast(v4u, v4f{dw[v][i], dw[v][i + 1], dw[v][i + 2], dw[v][i + 3]}));
+                to_b.store16(cx.column(v, i), __builtin_bit_cast(v4u, v4f{db[v][i], db[v][i + 1], db[v][i + 2], db[v][i + 3]}));
             }
         return;
     }
@@ -349,7 +349,10 @@ int launch_grad(int rows, int cols, const void* dy, int64_t lddy, const void* x,
     const norm_shape s = shape_of(cols, kVec<T>);
     const int row_waves = s.wave_row ? 1 : s.threads / kWave;
     const int teams = s.wave_row ? 8 : kNormMaxWaves / row_waves;
-    const int grid = std::min(grad_blocks(rows), static_cast<int>(ceil_div(rows, teams)));
+    // as many as make the same number of turns: no partial row is written for less (300 x 8192 BF16 13.6 us, with one
+    // workgroup per CU 15.7)
+    const int64_t per_turn = static_cast<int64_t>(std::max(1, grad_blocks(rows))) * teams;
+    const int grid = rows > 0 ? static_cast<int>(ceil_div(rows, ceil_div(rows, per_turn) * teams)) : 0;
     if (grid > 0) {
         const size_t lds = teams > 1 && partial ? 2 * sizeof(float) * s.nv * kVec<T> * (row_waves * kWave + 8) : 0;
         const bool all_dwords = rows_are_dwords(x, ldx, cols, sizeof(T)) && rows_are_dwords(dy, lddy, cols, sizeof(T)) &&

@@ -8,7 +8,6 @@ namespace hpcdnn {
 typedef _Float16 f16;
 typedef __bf16 bf16;
 typedef unsigned v4u __attribute__((ext_vector_type(4)));
-typedef unsigned v2u __attribute__((ext_vector_type(2)));
 
 // Values of T in 16 bytes: what one lane loads or stores at a time.
 template <class T>
@@ -40,17 +39,6 @@ __device__ __forceinline__ v4u load_part(const T* p, int n) {
     for (int i = 0; i < kVec<T> - 1; ++i)
         if (i < n) r.t[i] = p[i];
     return r.u;
-}
-template <class T>
-__device__ __forceinline__ void store_part(T* p, v4u v, int n) {
-    union {
-        v4u u;
-        T t[kVec<T>];
-    } r;
-    r.u = v;
-#pragma unroll
-    for (int i = 0; i < kVec<T> - 1; ++i)
-        if (i < n) p[i] = r.t[i];
 }
 
 // Vector at column `col` of a row of `cols` columns: whole, cut at the end of the row, or zeros behind it.
@@ -117,6 +105,9 @@ struct row_buffer {
     }
     __device__ __forceinline__ v4u load16(int col) const {
         return __builtin_amdgcn_raw_buffer_load_b128(rs, col * static_cast<int>(sizeof(T)), 0, 0);
+    }
+    __device__ __forceinline__ void store16(int col, v4u v) const {
+        __builtin_amdgcn_raw_buffer_store_b128(v, rs, col * static_cast<int>(sizeof(T)), 0, 0);
     }
     // non-temporal: a large result that nothing on the way reads again
     __device__ __forceinline__ void store16_once(int col, v4u v) const {

@@ -120,8 +120,9 @@ def check_grad(blas, rows, cols, dtype, wtype, seed, pad=0, weight=True, ws_fill
     sa, sc = gw.abs().mean(1, keepdim=True), (gw * xh).abs().mean(1, keepdim=True)
     tol = half(dtype) * ref.abs() + U * r64 * (36 * sa + 40 * sc * xh.abs() + 6 * gw.abs()) + (2.0 ** -25 if dtype == F16 else 0)
     assert torch.all((dx.double() - ref).abs() <= tol)
-    # a column is added along a workgroup's rows, then over the workgroups in eight runs: at most rows + 8 additions,
-    # beyond 1024 rows (rows / 256 workgroups) + (1024 / 8) + 8; the wave's own sums and the roundings of xh: 8 more
+    # a column is added along a team's rows, over the teams of a workgroup (at most 16) and over the workgroups (at most 256,
+    # in 32 runs of 8): at most rows + 16 additions that change a sum, beyond 256 rows rows / 256 + 16 + 8 + 32; the wave's
+    # own sums and the roundings of xh: 8 more.  Both are below
     k = min(rows, rows / 256 + 128) + 16
     for got, terms in ((dw, dy64 * xh), (db, dy64)):
         want = terms.sum(0)
@@ -135,6 +136,13 @@ def check_grad(blas, rows, cols, dtype, wtype, seed, pad=0, weight=True, ws_fill
 @pytest.mark.parametrize("dtype,wtype", [(F32, F32), (F16, F16), (F16, F32), (BF16, BF16), (BF16, F32)])
 def test_gradient(blas, rows, cols, dtype, wtype):
     check_grad(blas, rows, cols, dtype, wtype, rows * 11 + cols, pad=(rows + cols) % 3)
+
+
+@pytest.mark.parametrize("rows,cols", [(300, 8200), (259, 8195), (513, 5002), (40, 16384)])
+@pytest.mark.parametrize("dtype,wtype", [(F32, F32), (F16, F16), (BF16, F32)])
+def test_gradient_of_wide_rows(blas, rows, cols, dtype, wtype):
+    """One row to a workgroup at a time, more rows than workgroups and fewer."""
+    check_grad(blas, rows, cols, dtype, wtype, rows + cols, pad=(rows + cols) % 3)
 
 
 @pytest.mark.parametrize("rows,cols", [(300, 130), (40, 3000)])
