@@ -20,7 +20,8 @@ namespace hpcdnn {
 constexpr int kW4Cols = 32;                      // columns of one lane and load
 constexpr int kW4Piece = kW4Cols * kWave;        // columns of a wave and load
 constexpr int kW4MaxWaves = 16;                  // waves of a workgroup
-constexpr int kW4LdsBytes = 65536;
+constexpr int kW4LdsBytes = 65536;               // of a workgroup
+constexpr size_t kW4CuLdsBytes = 163840;         // of a CU
 
 template <class T>
 constexpr int kW4Parts = kW4Cols / kVec<T>;      // 16-byte parts of a lane's x
@@ -224,7 +225,7 @@ __global__ __launch_bounds__(kW4MaxWaves * kWave) void w4_gemv_kernel(int batch,
 // LDS at the end (in wave order): so a narrow matrix still keeps every CU loading.
 //
 // What limits it is the number of cache lines and 64-byte pieces that the loads touch: neighbouring lanes therefore load
-// neighbouring 16 bytes (four lanes a row's unit of weights, sixteen lanes a token's unit of x), and the order that the
+// neighbouring 16 bytes (four lanes a row's unit of weights, four lanes 64 bytes of a token), and the order that the
 // instructions want, row or token l % 16 and part l / 16 in lane l, comes about in LDS, each wave for itself.  (Loaded in that
 // order right away, thirteen tokens by 6143 x 8200 took 20 us; scales go through LDS as well, sixteen of a row at a time.)
 //
@@ -574,12 +575,15 @@ int launch_w4(int batch, int M, int N, int group_shift, float alpha, const unsig
         constexpr int TB = decltype(tb)::value, kRows = decltype(rows)::value, kPieces = kRows < 4 ? 4 / kRows : 1;
         const int panel = panel_of(N, TB, sizeof(T));
         const size_t lds = static_cast<size_t>(TB) * panel * sizeof(T) + static_cast<size_t>(TB) * panel / kW4Cols * sizeof(float);
-        // one workgroup of sixteen waves per CU; fewer waves while there are not enough rows for that
-        int waves = kW4MaxWaves;
-        while (waves > 4 && ceil_div(M, waves * kRows) < cus) waves /= 2;
+        // A CU holds sixteen waves.  As one workgroup they share x; as four of four waves, each with its own copy of x, they
+        // follow M more closely: taken where that spares the CU with the most rows more than a quarter of them and the copies
+        // fit (4149 x 8320 10.8 us, as one workgroup 11.4; 9000 x 2000 6.1 and 6.8; two copies of 9000 x 28672 37.1 and 33.8).
+        auto most_rows = [&](int w) { return ceil_div(ceil_div(M, w * kRows), cus) * w * kRows; };
+        const size_t copies = static_cast<size_t>(std::min<int64_t>(4, ceil_div(ceil_div(M, 4 * kRows), cus)));
+        const int waves = 4 * most_rows(4) < 3 * most_rows(kW4MaxWaves) && copies * lds <= kW4CuLdsBytes ? 4 : kW4MaxWaves;
         const int unit = waves * kRows;
         // x in several panels is staged for every round of rows: one round per workgroup then
-        const int per_block = panel < N ? unit : static_cast<int>(ceil_div(ceil_div(M, unit), cus)) * unit;
+        const int per_block = panel < N ? unit : static_cast<int>(ceil_div(ceil_div(M, unit), cus * (kW4MaxWaves / waves))) * unit;
         const dim3 grid(static_cast<unsigned>(ceil_div(M, per_block)), static_cast<unsigned>(ceil_div(batch, TB)));
         w4_gemv_kernel<T, TB, kRows, kPieces, kZeros><<<grid, waves * kWave, lds, stream>>>(
             batch, M, N, group_shift, alpha, q, ldq, static_cast<const T*>(scales), zeros, ldg, static_cast<const T*>(x), ldx, beta,

@@ -80,6 +80,13 @@ def test_single_token(blas, M, N, dtype, zeros, group):
     check(blas, 1, M, N, group, dtype, zeros, M + N, pad=(M + N) % 3)
 
 
+@pytest.mark.parametrize("batch,M", [(1, 4149), (2, 5001), (1, 9001), (2, 12300), (1, 16500), (3, 4200), (4, 8200), (16, 12500), (17, 4111)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_many_rows(blas, batch, M, dtype):
+    """Several rows to a wave and several turns to a workgroup, the last of them cut."""
+    check(blas, batch, M, 321, 64, dtype, True, M)
+
+
 @pytest.mark.parametrize("batch", [2, 3, 4, 5, 7, 8, 13, 16, 17, 33])
 @pytest.mark.parametrize("dtype,zeros,group", [(F32, True, 64), (F16, True, 128), (F16, False, 32), (BF16, True, 32), (BF16, False, 64), (BF16, False, 128)])
 def test_several_tokens(blas, batch, dtype, zeros, group):
