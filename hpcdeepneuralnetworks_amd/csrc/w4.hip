@@ -8,7 +8,8 @@
 //    in FP32 by two-term dot instructions; the offset is taken out per 32 columns, with the group's zero point,
 //      sum (q - z) x = sum (16 + q) x - (16 + z) sum x,
 //    and only then scaled.  The smallest power of two whose mantissa takes a nibble in both types keeps what cancels there
-//    within a factor of about five of the result.  FP32 tokens use byte-to-float conversions and q itself.
+//    within a factor of about five of the result.  FP32 tokens use byte-to-float conversions and q itself, on the matrix
+//    cores q - z, which BF16 holds, and three BF16 in the place of each FP32 value.
 //  - x lies in LDS in the order in which the lanes need it, its sums over 32 columns beside it.
 #include <algorithm>
 #include <cmath>
@@ -233,11 +234,15 @@ __global__ __launch_bounds__(kW4MaxWaves * kWave) void w4_gemv_kernel(int batch,
 // 4 x 4 transposition in four lane swaps): dword d is then columns 32 d + 8 (l / 16) ... of the unit, and every instruction
 // stays inside one group.  The sums over x that take out the offset of the nibbles come from the same instruction with a
 // matrix of ones.
+//
+// FP32 tokens are taken apart into three BF16 each, exactly, and multiplied by q - z, which BF16 holds: three instructions of
+// 32 columns in the place of eight of four columns, each twice as long, and the products are exact as well.  (Sixteen tokens
+// by 16384 x 16384 63 us, with the FP32 instruction 115; seven by 6143 x 8201 26 and 37.)
 constexpr int kW4Unit = 128;
 // Tokens from which this form is taken.  16-bit: two cost the other form 32 us on 16384 x 16384 and this one 35, four 45 and 36.
-// FP32 (instructions of four columns, an eighth of the rate): four by 8192 x 8192 22 and 31 us, seven by 6143 x 8201 48 and 37.
+// FP32: three by 16384 x 16384 53 us and 60, by 4224 x 9408 22 and 26; four by 9984 x 11287 75 and 38, by 8192 x 8192 25 and 22.
 template <class T>
-constexpr int kW4TileTokens = sizeof(T) == 2 ? 3 : 5;
+constexpr int kW4TileTokens = sizeof(T) == 2 ? 3 : 4;
 constexpr int kW4TileWaves = 8;
 constexpr int kW4Segment = 16;  // scales of a row that a wave keeps in LDS at a time
 template <class T>
@@ -260,6 +265,41 @@ __device__ __forceinline__ v4u transpose_quarters(v4u w) {
     const auto c = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
     const auto d = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
     return v4u{c[0], c[1], d[0], d[1]};
+}
+
+// Bits 16 ... 31 of eight FP32 values, which for values that BF16 holds is their conversion.
+__device__ __forceinline__ v4u upper_halves(const float (&f)[8]) {
+    v4u u;
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+        u[p] = __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, f[2 * p + 1]), __builtin_bit_cast(unsigned, f[2 * p]), 0x07060302u);
+    return u;
+}
+
+// Eight FP32 values as three BF16 each, which add up to them: 24 bits are eight of the value, eight of what is left and
+// eight of what is left then.
+__device__ __forceinline__ void three_bf16(v4u lo, v4u hi, v4u (&out)[3]) {
+    float f[8], left[8];
+    auto upper = [](float v) { return __builtin_bit_cast(float, __builtin_bit_cast(unsigned, v) & 0xffff0000u); };
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        f[i] = __builtin_bit_cast(float, static_cast<unsigned>(i < 4 ? lo[i & 3] : hi[i & 3]));
+        left[i] = f[i] - upper(f[i]);
+    }
+    out[0] = upper_halves(f);
+    out[1] = upper_halves(left);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) left[i] -= upper(left[i]);
+    out[2] = upper_halves(left);
+}
+
+// q - z of the eight nibbles of w: at most eight bits, so BF16 holds it.
+__device__ __forceinline__ v4u exact_weights(unsigned w, float z) {
+    const unsigned even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = static_cast<float>((((j & 1) ? odd : even) >> (8 * (j / 2))) & 0xffu) - z;
+    return upper_halves(f);
 }
 
 // LDS of a wave of the kernel below: its parts, or its sums at the end.
@@ -329,19 +369,16 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
 #pragma unroll
             for (int d = g * kGroupSteps; d < (g + 1) * kGroupSteps; ++d) {
                 if constexpr (kF32) {
-                    // eight instructions of four columns each, column 32 d + 8 (l / 16) + j; q - z is exact
+                    v4u xo[kTokTiles][3];
+#pragma unroll
+                    for (int t = 0; t < kTokTiles; ++t) three_bf16(xv[t][2 * d], xv[t][2 * d + 1], xo[t]);
 #pragma unroll
                     for (int r = 0; r < kRowTiles; ++r) {
-                        const unsigned even = wt[r][d] & 0x0f0f0f0fu, odd = (wt[r][d] >> 4) & 0x0f0f0f0fu;
+                        const v4u wq = exact_weights(wt[r][d], offset[r][g]);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float wj = static_cast<float>((((j & 1) ? odd : even) >> (8 * (j / 2))) & 0xffu) - offset[r][g];
+                        for (int t = 0; t < kTokTiles; ++t)
 #pragma unroll
-                            for (int t = 0; t < kTokTiles; ++t) {
-                                const float xj = __builtin_bit_cast(float, static_cast<unsigned>(xv[t][2 * d + j / 4][j & 3]));
-                                acc[t][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(xj, wj, acc[t][r], 0, 0, 0);
-                            }
-                        }
+                            for (int k = 0; k < 3; ++k) acc[t][r] = mfma_16x16x32<bf16>(xo[t][k], wq, acc[t][r]);
                     }
                 } else {
                     constexpr unsigned kOne = std::is_same_v<T, f16> ? 0x3C003C00u : 0x3F803F80u;
@@ -558,17 +595,32 @@ int launch_w4(int batch, int M, int N, int group_shift, float alpha, const unsig
         else tile(row_tiles, tok_tiles, integral_constant<int, 4>{});
     };
     if (batch >= kW4TileTokens<T> && N > 0) {
-        // Row tiles of a workgroup: every one of them reads all of x, which is what bounds this form (12 TB/s out of the
-        // caches), but the CUs have to be covered.  Thirteen tokens, one / two / four tiles: 4096 x 8192 9.8 / 12.3 /
-        // 17.8 us, 8192 x 8192 16.5 / 13.7 / 19.2 us, 16384 x 16384 (sixteen tokens) 58 / 43 / 39 us.  Thirty-two
-        // 16-bit tokens go as two tiles of one workgroup: 8192 x 8192 18.1 us, as two workgroups 21.0.
-        constexpr int kMostTok = sizeof(T) == 2 ? 2 : 1;
-        if (kMostTok == 2 && batch > 16) {
-            if (M > 16 * cus) of_group(integral_constant<int, 2>{}, integral_constant<int, kMostTok>{});
-            else of_group(integral_constant<int, 1>{}, integral_constant<int, kMostTok>{});
-        } else if (M > 48 * cus) of_group(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-        else if (M > 16 * cus) of_group(integral_constant<int, 2>{}, integral_constant<int, 1>{});
-        else of_group(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+        // Row tiles of a workgroup: it reads all of x once, which costs about as much as one of them, and the CU with the
+        // most workgroups decides.  (Thirteen tokens, one / two / three / four tiles: 4096 x 8192 9.8 / 12.3 / - / 17.8 us,
+        // 8192 x 8192 16.5 / 13.7 / 16.9 / 19.2 us; six by 9879 x 9920 25.0 / 30.5 / 23.9 / 28.4 us; sixteen by
+        // 16384 x 16384 64 / 44 / 53 / 39 us.)
+        auto cost = [&](int row_tiles, int tok_tiles) {
+            return ceil_div(ceil_div(M, 16 * row_tiles) * ceil_div(batch, 16 * tok_tiles), cus) * (row_tiles + 1);
+        };
+        auto by_cost = [&](auto most_rows, auto tok_tiles) {
+            constexpr int kTok = decltype(tok_tiles)::value, kMost = decltype(most_rows)::value;
+            int best = 1;
+            for (int r = 2; r <= kMost; ++r)
+                if (cost(r, kTok) <= cost(best, kTok)) best = r;
+            if (best == 1) of_group(integral_constant<int, 1>{}, tok_tiles);
+            else if (best == 2) of_group(integral_constant<int, 2>{}, tok_tiles);
+            else if constexpr (kMost > 2) {
+                if (best == 3) of_group(integral_constant<int, 3>{}, tok_tiles);
+                else of_group(integral_constant<int, 4>{}, tok_tiles);
+            }
+        };
+        // Thirty-two 16-bit tokens go as two tiles of one workgroup: 8192 x 8192 18.1 us, as two workgroups 21.0.
+        bool pairs = false;
+        if constexpr (sizeof(T) == 2) {
+            pairs = batch > 16;
+            if (pairs) by_cost(integral_constant<int, 2>{}, integral_constant<int, 2>{});
+        }
+        if (!pairs) by_cost(integral_constant<int, 4>{}, integral_constant<int, 1>{});
         return launch_status();
     }
     auto go = [&](auto tb, auto rows) {
@@ -589,8 +641,8 @@ int launch_w4(int batch, int M, int N, int group_shift, float alpha, const unsig
             batch, M, N, group_shift, alpha, q, ldq, static_cast<const T*>(scales), zeros, ldg, static_cast<const T*>(x), ldx, beta,
             static_cast<T*>(y), ldy, per_block, panel);
     };
-    // Rows per wave and step: as many as leave every CU its sixteen waves.  Four FP32 tokens take x in panels, staged anew for
-    // every round of rows, so there two rows pay earlier: seven tokens by 6143 x 8201 41 us, with one row 56.
+    // Rows per wave and step: as many as leave every CU its sixteen waves.  Three FP32 tokens take x in panels, staged anew for
+    // every round of rows, so there two rows pay earlier: 5000 x 5001 16.2 us, with one row 23.7.
     auto by_rows = [&](auto tb, int two_rows_from) {
         if (M >= 64 * cus) go(tb, integral_constant<int, 4>{});
         else if (M >= two_rows_from * cus) go(tb, integral_constant<int, 2>{});
@@ -598,7 +650,7 @@ int launch_w4(int batch, int M, int N, int group_shift, float alpha, const unsig
     };
     if (batch == 1) by_rows(integral_constant<int, 1>{}, 32);
     else if (batch == 2 || sizeof(T) == 2) by_rows(integral_constant<int, 2>{}, 32);
-    else if constexpr (sizeof(T) == 4) by_rows(integral_constant<int, 4>{}, 16);
+    else if constexpr (sizeof(T) == 4) by_rows(integral_constant<int, 3>{}, 16);
     return launch_status();
 }
 

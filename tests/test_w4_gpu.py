@@ -4,7 +4,8 @@ Bound.  With u = 2^-24, the products (16 + q) x (q x for FP32 tokens) are exact 
 32 columns of one group, in the worst case with one rounding of at most u times (31 or 15) sum|x| per column and one each
 for the offset's sum and product: 36 u (o + 15 + o + z) sum|x|, o = 16 (0), below 36 * 62 u (36 * 30 u) sum|x| times |s|.
 The matrix-core form adds whole groups of up to 128 columns, in the worst case one rounding per column: 132 in the place of
-36, and for FP32 tokens (five and more) on q - z itself, of magnitude 15 at most, in the place of 30.  Adding the groups is off by u (N / 32 + 16) sum |s| (q - z) |x|, then the result is rounded once."""
+36.  FP32 tokens (four and more) go there as three parts each, of one sign, which add up to them: 3 * 128 exact products with
+q - z, of magnitude 15 at most, so 388 in the place of 36 and 15 in the place of 30.  Adding the groups is off by u (N / 32 + 16) sum |s| (q - z) |x|, then the result is rounded once."""
 import pytest
 import torch
 
@@ -56,7 +57,7 @@ def check(blas, batch, M, N, group, dtype, zeros, seed, alpha=1.0, beta=0.0, ldq
     w, ss = dense(q, s, z, M, N, group)
     x64 = x.double()
     ref = alpha * (x64 @ (w * ss).t().contiguous())
-    worst = (132 * 62 if dtype != F32 else 132 * 15 if batch >= 5 else 36 * 30) * (x64.abs() @ ss.abs().t().contiguous()) + (N / 32 + 16) * (x64.abs() @ (w * ss).abs().t().contiguous())
+    worst = (132 * 62 if dtype != F32 else 388 * 15 if batch >= 4 else 36 * 30) * (x64.abs() @ ss.abs().t().contiguous()) + (N / 32 + 16) * (x64.abs() @ (w * ss).abs().t().contiguous())
     if beta != 0:
         ref = ref + beta * y0
     tol = half(dtype) * ref.abs() + U * (abs(alpha) * worst + 3 * ref.abs() + (abs(beta) * y0.abs() if beta != 0 else 0))
@@ -142,6 +143,36 @@ def test_infinite_and_missing_numbers_stay_in_their_token(blas, batch):
     y = torch.empty(batch + 1, 40, dtype=BF16, device="cuda")
     blas.w4_gemv(batch + 1, 40, 300, 64, 1.0, q, s, None, x, 0.0, y)
     assert torch.all(torch.isnan(y[-1])) and torch.all(torch.isfinite(y[:-1]))
+
+
+@pytest.mark.parametrize("batch", [1, 2, 3, 4, 7])
+def test_missing_numbers_of_fp32_tokens(blas, batch):
+    """Every infinity and NaN, also one whose upper bits alone are an infinity's, stays in its token and reaches all of it."""
+    q, s, _ = make(40, 300, 64, F32, False, 12)
+    for bits in (0x7F800000, 0x7F800001, 0x7FC00000, -0x7FFFFF):   # the last: a NaN of negative sign
+        x = torch.randn(batch + 1, 300, device="cuda")
+        x.view(torch.int32)[-1, 7] = bits
+        y = torch.empty(batch + 1, 40, device="cuda")
+        blas.w4_gemv(batch + 1, 40, 300, 64, 1.0, q, s, None, x, 0.0, y)
+        assert not torch.any(torch.isfinite(y[-1])) and torch.all(torch.isfinite(y[:-1]))
+
+
+@pytest.mark.parametrize("batch", [1, 3, 4, 16])
+@pytest.mark.parametrize("exponent", [-130, -118, -105, 60, 121])
+def test_range_of_fp32_tokens(blas, batch, exponent):
+    """Values far below one lose at most what is under 2^-133 each, large ones nothing, up to a factor of 64 below the largest."""
+    M, N, group = 48, 700, 64
+    q, _, _ = make(M, N, group, F32, False, 13)
+    s = torch.rand(M, -(-N // group), device="cuda") * 0.02 + 0.01   # below 0.03: sums of 700 stay below 2^127
+    g = torch.Generator().manual_seed(14)
+    x = (torch.rand(batch, N, generator=g) * 2 - 1).mul(2.0 ** exponent).cuda()
+    y = torch.empty(batch, M, device="cuda")
+    blas.w4_gemv(batch, M, N, group, 1.0, q, s, None, x, 0.0, y)
+    w, ss = dense(q, s, None, M, N, group)
+    ref = x.double() @ (w * ss).t().contiguous()
+    worst = (388 * 15 if batch >= 4 else 36 * 30) * (x.double().abs() @ ss.abs().t().contiguous()) + (N / 32 + 16) * (x.double().abs() @ (w * ss).abs().t().contiguous())
+    tiny = (2.0 ** -133 * 15 + 2.0 ** -148 * 4) * N * 0.03 + 2.0 ** -148 * N   # and results that are subnormal themselves
+    assert torch.all((y.double() - ref).abs() <= U * (worst + 3 * ref.abs()) + tiny)
 
 
 def test_packed_by_the_host_function(blas):
