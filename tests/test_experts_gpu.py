@@ -90,7 +90,8 @@ def rows(n, cols, dtype, seed, pad=0):
     return buf[:, :cols], buf
 
 
-SIZES = [(1, 1, 1, 1), (3, 2, 4, 8), (7, 8, 16, 1001), (50, 3, 9, 2048), (20, 4, 8, 2050), (33, 2, 64, 4096), (5, 6, 8, 16385), (300, 5, 6, 40), (9, 64, 70, 96)]
+SIZES = [(1, 1, 1, 1), (3, 2, 4, 8), (7, 8, 16, 1001), (50, 3, 9, 2048), (20, 4, 8, 2050), (33, 2, 64, 4096), (5, 6, 8, 16385), (300, 5, 6, 40), (9, 64, 70, 96),
+         (6, 1, 3, 2050), (7, 1, 4, 1001), (61, 1, 5, 200), (33, 1, 4, 3), (1030, 1, 9, 4100)]
 
 
 @pytest.mark.parametrize("tokens,topk,experts,cols", SIZES)
