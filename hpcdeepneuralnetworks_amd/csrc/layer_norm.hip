@@ -297,10 +297,10 @@ struct norm_shape {
     bool wave_row;
     int nv, threads;
 };
-norm_shape shape_of(int cols, int vec) {
+norm_shape shape_of(int cols, int vec, int least_nv = 1) {
     const int vecs = static_cast<int>(ceil_div(cols, vec));
     if (vecs <= 2 * kWave) return {true, vecs <= kWave ? 1 : 2, kNormRowWaves * kWave};
-    const int nv = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4;
+    const int nv = std::max(least_nv, vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4);
     return {false, nv, static_cast<int>(ceil_div(ceil_div(vecs, nv), kWave)) * kWave};
 }
 
@@ -346,7 +346,12 @@ int launch_norm(int rows, int cols, const void* x, int64_t ldx, const void* w, c
 template <class T, class W>
 int launch_grad(int rows, int cols, const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, const float* mean,
                 const float* rstd, void* dx, int64_t lddx, void* dw, void* db, float* partial, hipStream_t stream) {
-    const norm_shape s = shape_of(cols, kVec<T>);
+    norm_shape s = shape_of(cols, kVec<T>);
+    // Nine or ten waves to a row leave a CU's workgroup at that; with two vectors per thread it is three teams of five.  Only
+    // many rows make up for the longer turn: 5000 x 5001 BF16 41 us instead of 49, 16384 x 4160 91 instead of 99, but
+    // 1000 x 5000 17.2 instead of 16.3.
+    if (!s.wave_row && s.nv == 1 && s.threads > 8 * kWave && s.threads <= 10 * kWave && rows >= 8 * device_cus())
+        s = shape_of(cols, kVec<T>, 2);
     const int row_waves = s.wave_row ? 1 : s.threads / kWave;
     const int teams = s.wave_row ? 8 : kNormMaxWaves / row_waves;
     // as many as make the same number of turns: no partial row is written for less (300 x 8192 BF16 13.6 us, with one

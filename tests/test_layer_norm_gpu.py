@@ -138,10 +138,10 @@ def test_gradient(blas, rows, cols, dtype, wtype):
     check_grad(blas, rows, cols, dtype, wtype, rows * 11 + cols, pad=(rows + cols) % 3)
 
 
-@pytest.mark.parametrize("rows,cols", [(300, 8200), (259, 8195), (513, 5002), (40, 16384)])
+@pytest.mark.parametrize("rows,cols", [(300, 8200), (259, 8195), (513, 5002), (40, 16384), (2050, 4203), (2333, 2306), (2100, 4800)])
 @pytest.mark.parametrize("dtype,wtype", [(F32, F32), (F16, F16), (BF16, F32)])
 def test_gradient_of_wide_rows(blas, rows, cols, dtype, wtype):
-    """One row to a workgroup at a time, more rows than workgroups and fewer."""
+    """One row to a workgroup at a time, more rows than workgroups and fewer; nine waves to a row and many rows."""
     check_grad(blas, rows, cols, dtype, wtype, rows + cols, pad=(rows + cols) % 3)
 
 
