@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
 #include <type_traits>
 
 #include "hpcdnn.h"
@@ -34,6 +35,28 @@ inline int device_cus() {
         cus[dev] = n;
     }
     return cus[dev];
+}
+
+// Kernels that use more than the default 64 KiB of LDS must opt in once per device.
+inline int enable_lds(const void* fn, size_t bytes) {
+    if (bytes <= 64 * 1024) return HPCDNN_OK;
+    struct Done {
+        const void* fn;
+        int device;
+    };
+    static std::mutex mu;
+    static Done done[512] = {};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return static_cast<int>(e);
+    std::lock_guard<std::mutex> lock(mu);
+    for (const Done& d : done)
+        if (d.fn == fn && d.device == dev) return HPCDNN_OK;
+    e = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    if (e != hipSuccess) return static_cast<int>(e);
+    for (Done& d : done)
+        if (!d.fn) { d = Done{fn, dev}; break; }  // a full table only costs a repeated call
+    return HPCDNN_OK;
 }
 
 // ---- counter-based RNG: splitmix64 finaliser of seed*golden + index ------

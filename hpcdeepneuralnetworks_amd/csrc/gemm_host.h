@@ -1,7 +1,6 @@
 // Host-side helpers shared by the SGEMM and ABFT-SGEMM entry points.
 #pragma once
 
-#include <mutex>
 
 #include "sgemm_kernel.h"
 
@@ -89,27 +88,6 @@ HPCDNN_FT_DECLARE(3)
 HPCDNN_FT_DECLARE(4)
 #undef HPCDNN_FT_DECLARE
 
-// Kernels that use more than the default 64 KiB of LDS must opt in once per device.
-inline int enable_lds(void (*fn)(const GemmArgs), size_t bytes) {
-    if (bytes <= 64 * 1024) return HPCDNN_OK;
-    struct Done {
-        const void* fn;
-        int device;
-    };
-    static std::mutex mu;
-    static Done done[512] = {};
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return static_cast<int>(e);
-    std::lock_guard<std::mutex> lock(mu);
-    const void* key = reinterpret_cast<const void*>(fn);
-    for (const Done& d : done)
-        if (d.fn == key && d.device == dev) return HPCDNN_OK;
-    e = hipFuncSetAttribute(key, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-    if (e != hipSuccess) return static_cast<int>(e);
-    for (Done& d : done)
-        if (!d.fn) { d = Done{key, dev}; break; }  // a full table only costs a repeated call
-    return HPCDNN_OK;
-}
+inline int enable_lds(void (*fn)(const GemmArgs), size_t bytes) { return enable_lds(reinterpret_cast<const void*>(fn), bytes); }
 
 }  // namespace hpcdnn

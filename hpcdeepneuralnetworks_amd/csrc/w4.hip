@@ -21,8 +21,7 @@ namespace hpcdnn {
 constexpr int kW4Cols = 32;                      // columns of one lane and load
 constexpr int kW4Piece = kW4Cols * kWave;        // columns of a wave and load
 constexpr int kW4MaxWaves = 16;                  // waves of a workgroup
-constexpr int kW4LdsBytes = 65536;               // of a workgroup
-constexpr size_t kW4CuLdsBytes = 163840;         // of a CU
+constexpr size_t kW4LdsBytes = 163840;           // of a CU
 
 template <class T>
 constexpr int kW4Parts = kW4Cols / kVec<T>;      // 16-byte parts of a lane's x
@@ -565,7 +564,8 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
 
 namespace {
 
-// Columns of x that LDS holds for TB tokens, a multiple of 2048; panels of equal size where one does not hold all.
+// Columns of x that LDS holds for TB tokens, a multiple of 2048; panels of equal size where one does not hold all.  A
+// workgroup may take all of a CU's LDS (two FP32 tokens by 4224 x 9408 17 us, in two panels of 64 KiB at most 26).
 int panel_of(int N, int tb, size_t elem) {
     const int most = static_cast<int>(kW4LdsBytes / (tb * (kW4Piece * elem + kWave * sizeof(float))));
     const int pieces = std::max(1, static_cast<int>(ceil_div(N, kW4Piece)));
@@ -632,26 +632,30 @@ int launch_w4(int batch, int M, int N, int group_shift, float alpha, const unsig
         // fit (4149 x 8320 10.8 us, as one workgroup 11.4; 9000 x 2000 6.1 and 6.8; two copies of 9000 x 28672 37.1 and 33.8).
         auto most_rows = [&](int w) { return ceil_div(ceil_div(M, w * kRows), cus) * w * kRows; };
         const size_t copies = static_cast<size_t>(std::min<int64_t>(4, ceil_div(ceil_div(M, 4 * kRows), cus)));
-        const int waves = 4 * most_rows(4) < 3 * most_rows(kW4MaxWaves) && copies * lds <= kW4CuLdsBytes ? 4 : kW4MaxWaves;
+        const int waves = 4 * most_rows(4) < 3 * most_rows(kW4MaxWaves) && copies * lds <= kW4LdsBytes ? 4 : kW4MaxWaves;
         const int unit = waves * kRows;
         // x in several panels is staged for every round of rows: one round per workgroup then
         const int per_block = panel < N ? unit : static_cast<int>(ceil_div(ceil_div(M, unit), cus * (kW4MaxWaves / waves))) * unit;
         const dim3 grid(static_cast<unsigned>(ceil_div(M, per_block)), static_cast<unsigned>(ceil_div(batch, TB)));
-        w4_gemv_kernel<T, TB, kRows, kPieces, kZeros><<<grid, waves * kWave, lds, stream>>>(
+        auto* const fn = &w4_gemv_kernel<T, TB, kRows, kPieces, kZeros>;
+        if (lds > 64 * 1024)
+            if (int e = enable_lds(reinterpret_cast<const void*>(fn), kW4LdsBytes)) return e;
+        fn<<<grid, waves * kWave, lds, stream>>>(
             batch, M, N, group_shift, alpha, q, ldq, static_cast<const T*>(scales), zeros, ldg, static_cast<const T*>(x), ldx, beta,
             static_cast<T*>(y), ldy, per_block, panel);
+        return launch_status();
     };
-    // Rows per wave and step: as many as leave every CU its sixteen waves.  Three FP32 tokens take x in panels, staged anew for
-    // every round of rows, so there two rows pay earlier: 5000 x 5001 16.2 us, with one row 23.7.
+    // Rows per wave and step: as many as leave every CU its sixteen waves.  Three FP32 tokens are bound by reading x from LDS,
+    // so there two rows pay earlier: 8000 x 8192 21.4 us, with one row 23.0.
     auto by_rows = [&](auto tb, int two_rows_from) {
-        if (M >= 64 * cus) go(tb, integral_constant<int, 4>{});
-        else if (M >= two_rows_from * cus) go(tb, integral_constant<int, 2>{});
-        else go(tb, integral_constant<int, 1>{});
+        if (M >= 64 * cus) return go(tb, integral_constant<int, 4>{});
+        if (M >= two_rows_from * cus) return go(tb, integral_constant<int, 2>{});
+        return go(tb, integral_constant<int, 1>{});
     };
-    if (batch == 1) by_rows(integral_constant<int, 1>{}, 32);
-    else if (batch == 2 || sizeof(T) == 2) by_rows(integral_constant<int, 2>{}, 32);
-    else if constexpr (sizeof(T) == 4) by_rows(integral_constant<int, 3>{}, 16);
-    return launch_status();
+    if (batch == 1) return by_rows(integral_constant<int, 1>{}, 32);
+    if constexpr (sizeof(T) == 4)
+        if (batch > 2) return by_rows(integral_constant<int, 3>{}, 16);
+    return by_rows(integral_constant<int, 2>{}, 32);
 }
 
 int shift_of(int group) { return group == 32 ? 5 : group == 64 ? 6 : group == 128 ? 7 : -1; }
