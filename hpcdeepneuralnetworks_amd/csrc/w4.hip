@@ -11,6 +11,7 @@
 //    within a factor of about five of the result.  FP32 tokens use byte-to-float conversions and q itself, on the matrix
 //    cores q - z, which BF16 holds, and three BF16 in the place of each FP32 value.
 //  - x lies in LDS in the order in which the lanes need it, its sums over 32 columns beside it.
+// Measured, one token: 16384 x 16384 FP16 in groups of 64 with zero points 28 us (5.2 TB/s), 4096 x 4096 BF16 5.3 us.
 #include <algorithm>
 #include <cmath>
 
