@@ -33,7 +33,7 @@ __device__ __forceinline__ v4u pair_order(v4u d) {
                __builtin_amdgcn_perm(d[3], d[1], 0x05040100u), __builtin_amdgcn_perm(d[3], d[1], 0x07060302u)};
 }
 
-// The eight nibbles of w as 16 + q in T, columns (p, p + 4) in dword p: a shift and one v_bfi_b32 each.  An instruction takes
+// The eight nibbles of w as 16 + q in T, columns (p, p + 4) in dword p: a shift and an and-or each.  An instruction takes
 // one constant from a scalar register and none from the instruction stream beside it, so the second has to be a vector
 // register; left to itself the compiler uses two instructions with a literal each instead.
 template <class T>
