@@ -88,10 +88,16 @@ __global__ __launch_bounds__(kSortMaxThreads) void expert_place_kernel(unsigned 
         const int e = threadIdx.x & ((1 << bits) - 1), shares = blockDim.x >> bits, share = threadIdx.x >> bits;
         if (e < experts && share < shares) {
             int all = 0, earlier = 0;
-            for (int b = share; b < blocks; b += shares) {
-                const int c = counts[b * experts + e];
-                all += c;
-                if (b < static_cast<int>(blockIdx.x)) earlier += c;
+            // eight loads on their way at a time: 83968 choices of 223 experts 8.8 us, one after the other 12.3
+            for (int b0 = share; b0 < blocks; b0 += 8 * shares) {
+                int c[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) c[u] = b0 + u * shares < blocks ? counts[(b0 + u * shares) * experts + e] : 0;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    all += c[u];
+                    if (b0 + u * shares < static_cast<int>(blockIdx.x)) earlier += c[u];
+                }
             }
             atomicAdd(&total[e], all);
             atomicAdd(&before[e], earlier);
