@@ -408,12 +408,12 @@ __global__ __launch_bounds__(kW4TileWaves * kWave) void w4_tile_kernel(int batch
                     }
         }
     };
-    // Part p of row i stands at (p ^ i / 4): sixteen lanes meet no bank twice, neither writing nor reading.  A wave's LDS
-    // accesses are carried out in order, so one place does for all.
+    // Part p of row i stands at (p ^ i / 2 % 4): eight lanes meet no bank twice, neither writing nor reading (a third of the
+    // conflicts counted with i / 4 or without).  A wave's LDS accesses are carried out in order, so one place does for all.
     auto to_instruction_order = [&](v4u v) {
-        *reinterpret_cast<v4u*>(mine + load_row_of * 64 + ((load_part ^ (load_row_of >> 2)) & 3) * 16) = v;
+        *reinterpret_cast<v4u*>(mine + load_row_of * 64 + ((load_part ^ (load_row_of >> 1)) & 3) * 16) = v;
         __builtin_amdgcn_wave_barrier();
-        const v4u got = *reinterpret_cast<const v4u*>(mine + row * 64 + ((quarter ^ (row >> 2)) & 3) * 16);
+        const v4u got = *reinterpret_cast<const v4u*>(mine + row * 64 + ((quarter ^ (row >> 1)) & 3) * 16);
         __builtin_amdgcn_wave_barrier();
         return got;
     };
