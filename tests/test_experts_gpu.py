@@ -114,7 +114,8 @@ def test_gather(blas, tokens, topk, experts, cols, dtype):
     assert torch.equal(short[:few], x[order[:few].long() // topk]) and torch.equal(short[few:], keep[few:])
 
 
-@pytest.mark.parametrize("tokens,topk,experts,cols", SIZES)
+# beside those: a token's choices in one workgroup of the gradient, and in two
+@pytest.mark.parametrize("tokens,topk,experts,cols", SIZES + [(5000, 5, 20, 1030), (3000, 5, 20, 2051)])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("weighted", [True, False])
 def test_combine_and_gradient(blas, tokens, topk, experts, cols, dtype, weighted):
