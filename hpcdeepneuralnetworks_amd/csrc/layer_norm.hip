@@ -42,9 +42,12 @@ __device__ __forceinline__ void load_params(const W* p, float fill, const row_va
 }
 
 // One row per wave (kWaveRow: no exchange between waves) or per workgroup.  The mean and the squared deviations of a
-// wave's part of the row are formed in two passes over registers, the parts then joined exactly,
-//   mu = sum n_w mu_w / C,   M2 = sum M2_w + n_w (mu_w - mu)^2,
+// wave's part of the row are formed in two passes over registers, the parts then joined,
+//   mu = mu_0 + sum n_w (mu_w - mu_0) / C,   M2 = sum M2_w + n_w (mu_w - mu)^2,
 // so nothing cancels (sum x^2 - C mu^2 would lose the variance of rows with a large mean) and a row costs one barrier.
+// A sum of equal FP32 values rounds, and its mean may be some steps beside them; their deviations from it are exact and few
+// steps large, so these add up exactly, and the mean is moved by what they leave: a row of equal values has exactly
+// that mean, and no spread.  (16-bit values have room in the sum of a wave, and only the join needs its shift by mu_0.)
 // The next row is loaded into the registers of the present one as soon as that is unpacked.
 template <class T, class W, int NV, bool kWaveRow, row_kind kKind>
 __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer_norm_kernel(
@@ -68,8 +71,12 @@ __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer
     for (int v = 0; v < NV; ++v)
 #pragma unroll
         for (int i = 0; i < kVec<T>; ++i) valid += cur.own(v, i);
-    const float n_wave = wave_allsum(static_cast<float>(valid));
+    const float n_wave = wave_allsum(static_cast<float>(valid));  // at least one
     const float n_cols = static_cast<float>(cols);
+    // v / n.  16-bit rows divide: their wave's sum of equal values is exact, and then so is its mean.  FP32 rows multiply, which
+    // makes up for the sum that corrects their mean (16384 x 4096 84.0 us with and without it, 85.8 with it and divisions).
+    const float inv_wave = 1.f / n_wave, inv_cols = 1.f / n_cols;
+    auto over = [](float v, float n, float inv) { return std::is_same_v<T, float> ? v * inv : v / n; };
     // columns of wave (lane & 15): what the join below weighs that wave's mean with
     float n_of_lane = 0.f;
     if (!kWaveRow) {
@@ -87,16 +94,25 @@ __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) sum += kKind != kOverlapRows || cur.own(v, i) ? f[v][i] : 0.f;  // (zeros behind the end)
-        // divided, not multiplied by a reciprocal: a row of equal values then has exactly that mean, and no spread
-        float mu = wave_allsum(sum) / fmaxf(n_wave, 1.f), m2 = 0.f;
+        float mu = over(wave_allsum(sum), n_wave, inv_wave), m2 = 0.f;
+        [[maybe_unused]] float left = 0.f;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int i = 0; i < kVec<T>; ++i) {
                 const float d = cur.own(v, i) ? f[v][i] - mu : 0.f;
                 m2 = __builtin_fmaf(d, d, m2);
+                if constexpr (std::is_same_v<T, float>) left += d;
             }
         m2 = wave_allsum(m2);
+        if constexpr (std::is_same_v<T, float>) {
+            left = wave_allsum(left);
+            const float shift = left * inv_wave;
+            if (__builtin_fabsf(left) < __builtin_inff()) {  // (beside an infinity there is nothing to move)
+                mu += shift;
+                m2 = __builtin_fmaxf(__builtin_fmaf(-left, shift, m2), 0.f);
+            }
+        }
         if (!kWaveRow) {
             if (lane == 0) {
                 part[turn][0][wave] = mu;
@@ -104,11 +120,13 @@ __global__ __launch_bounds__(kWaveRow ? kNormRowWaves * kWave : 1024) void layer
             }
             __syncthreads();
             const bool has = (lane & 15) < waves;
+            const float mu_0 = part[turn][0][0];
             const float mu_w = has ? part[turn][0][lane & 15] : 0.f, m2_w = has ? part[turn][1][lane & 15] : 0.f;
-            mu = row16_allsum(n_of_lane * mu_w) / n_cols;
+            mu = mu_0 + over(row16_allsum(n_of_lane * (mu_w - mu_0)), n_cols, inv_cols);
+            if (!(__builtin_fabsf(mu) < __builtin_inff())) mu = row16_allsum(n_of_lane * mu_w) / n_cols;  // the mean of a row with an infinity is one
             m2 = row16_allsum(__builtin_fmaf(n_of_lane * (mu_w - mu), mu_w - mu, m2_w));
         }
-        const float rs = 1.f / __builtin_sqrtf(m2 / n_cols + eps);
+        const float rs = 1.f / __builtin_sqrtf(over(m2, n_cols, inv_cols) + eps);
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
