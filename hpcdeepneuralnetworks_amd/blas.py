@@ -422,6 +422,26 @@ def _flat(t: torch.Tensor | None, n: int, name: str, dtype: torch.dtype, dev: in
     return t.data_ptr()
 
 
+def _choices(t: torch.Tensor | None, tokens: int, topk: int, name: str, dtype: torch.dtype, dev: int):
+    """Pointer of a value per choice: rows of topk values without gaps, or all of them in one dimension."""
+    p = _flat(t, tokens * topk, name, dtype, dev)
+    if p is not None:
+        shape = t.shape
+        if len(shape) > 1 and shape[-1] != topk and t.numel() != max(shape):
+            raise HpcdnnError(f"{name} must have rows of {topk} values, got {tuple(shape)}")
+    return p
+
+
+def _per_row(t: torch.Tensor | None, rows: int, name: str, dev: int):
+    """Pointer of a float32 value per row."""
+    p = _flat(t, rows, name, torch.float32, dev)
+    if p is not None:
+        shape = t.shape
+        if len(shape) > 1 and t.numel() != rows and t.numel() != max(shape):
+            raise HpcdnnError(f"{name} must have one value per row, got {tuple(shape)}")
+    return p
+
+
 def _scratch(ws: torch.Tensor | None, dev: int):
     if ws is None:
         return None, 0
@@ -452,7 +472,7 @@ def layer_norm(rows: int, cols: int, x: torch.Tensor, w: torch.Tensor | None, b:
     py, ldy = _rows(y, rows, cols, "y", x.dtype, dev)
     pt = _param_type((w, b), x.dtype)
     check(_lib.lib().hpcdnn_layer_norm(t, _TYPES[pt], rows, cols, px, ldx, _flat(w, cols, "w", pt, dev), _flat(b, cols, "b", pt, dev), eps, py, ldy,
-                                       _flat(mean, rows, "mean", torch.float32, dev), _flat(rstd, rows, "rstd", torch.float32, dev), _stream_of(dev)),
+                                       _per_row(mean, rows, "mean", dev), _per_row(rstd, rows, "rstd", dev), _stream_of(dev)),
           "hpcdnn_layer_norm")
 
 
@@ -469,7 +489,7 @@ def layer_norm_grad(rows: int, cols: int, dy: torch.Tensor, x: torch.Tensor, w: 
     pt = _param_type((w, dw, db), x.dtype)
     wp, wb = _scratch(ws, dev)
     check(_lib.lib().hpcdnn_layer_norm_grad(t, _TYPES[pt], rows, cols, pdy, lddy, px, ldx, _flat(w, cols, "w", pt, dev),
-                                            _flat(mean, rows, "mean", torch.float32, dev), _flat(rstd, rows, "rstd", torch.float32, dev), pdx, lddx,
+                                            _per_row(mean, rows, "mean", dev), _per_row(rstd, rows, "rstd", dev), pdx, lddx,
                                             _flat(dw, cols, "dw", pt, dev), _flat(db, cols, "db", pt, dev), wp, wb, _stream_of(dev)),
           "hpcdnn_layer_norm_grad")
 
@@ -529,7 +549,7 @@ def expert_sort(tokens: int, topk: int, experts: int, ids: torch.Tensor, offsets
     pi, ldi = _rows(ids, tokens, topk, "ids", torch.int32, dev)
     wp, wb = _scratch(ws, dev)
     check(_lib.lib().hpcdnn_expert_sort(tokens, topk, experts, pi, ldi, _flat(offsets, experts + 1, "offsets", torch.int32, dev),
-                                        _flat(pos, tokens * topk, "pos", torch.int32, dev), _flat(order, tokens * topk, "order", torch.int32, dev),
+                                        _choices(pos, tokens, topk, "pos", torch.int32, dev), _flat(order, tokens * topk, "order", torch.int32, dev),
                                         wp, wb, _stream_of(dev)), "hpcdnn_expert_sort")
 
 
@@ -543,7 +563,7 @@ def expert_gather(tokens: int, topk: int, rows: int, cols: int, x: torch.Tensor,
     dev = _device(x, "x")
     px, ldx = _rows(x, tokens, cols, "x", x.dtype, dev)
     po, ldo = _rows(out, rows, cols, "out", x.dtype, dev)
-    check(_lib.lib().hpcdnn_expert_gather(t, tokens, topk, rows, cols, px, ldx, _flat(pos, tokens * topk, "pos", torch.int32, dev), po, ldo,
+    check(_lib.lib().hpcdnn_expert_gather(t, tokens, topk, rows, cols, px, ldx, _choices(pos, tokens, topk, "pos", torch.int32, dev), po, ldo,
                                           _stream_of(dev)), "hpcdnn_expert_gather")
 
 
@@ -555,8 +575,8 @@ def expert_combine(tokens: int, topk: int, rows: int, cols: int, xs: torch.Tenso
     dev = _device(xs, "xs")
     px, ldx = _rows(xs, rows, cols, "xs", xs.dtype, dev)
     py, ldy = _rows(y, tokens, cols, "y", xs.dtype, dev)
-    check(_lib.lib().hpcdnn_expert_combine(t, tokens, topk, rows, cols, px, ldx, _flat(pos, tokens * topk, "pos", torch.int32, dev),
-                                           _flat(weights, tokens * topk, "weights", torch.float32, dev), py, ldy, _stream_of(dev)),
+    check(_lib.lib().hpcdnn_expert_combine(t, tokens, topk, rows, cols, px, ldx, _choices(pos, tokens, topk, "pos", torch.int32, dev),
+                                           _choices(weights, tokens, topk, "weights", torch.float32, dev), py, ldy, _stream_of(dev)),
           "hpcdnn_expert_combine")
 
 
@@ -570,9 +590,9 @@ def expert_combine_grad(tokens: int, topk: int, rows: int, cols: int, dy: torch.
     px, ldx = _rows(xs, rows, cols, "xs", dy.dtype, dev) if dweights is not None else (None, cols)
     pdx, lddx = _rows(dxs, rows, cols, "dxs", dy.dtype, dev) if dxs is not None else (None, cols)
     check(_lib.lib().hpcdnn_expert_combine_grad(t, tokens, topk, rows, cols, pdy, lddy, px, ldx,
-                                                _flat(pos, tokens * topk, "pos", torch.int32, dev),
-                                                _flat(weights, tokens * topk, "weights", torch.float32, dev), pdx, lddx,
-                                                _flat(dweights, tokens * topk, "dweights", torch.float32, dev), _stream_of(dev)),
+                                                _choices(pos, tokens, topk, "pos", torch.int32, dev),
+                                                _choices(weights, tokens, topk, "weights", torch.float32, dev), pdx, lddx,
+                                                _choices(dweights, tokens, topk, "dweights", torch.float32, dev), _stream_of(dev)),
           "hpcdnn_expert_combine_grad")
 
 

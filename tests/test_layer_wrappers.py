@@ -1,0 +1,96 @@
+"""What the tensor wrappers of the layer operators pass on and what they refuse, with a library that only records its calls."""
+import pytest
+import torch
+
+from hpcdeepneuralnetworks_amd import blas
+
+
+class OnGpu(torch.Tensor):
+    """A host tensor that says it lives on GPU 0; nothing looks at its values."""
+    is_cuda = True
+
+    def get_device(self):
+        return 0
+
+
+def gpu(t):
+    return t.as_subclass(OnGpu)
+
+
+def zeros(*shape, dtype=torch.float32):
+    return gpu(torch.zeros(*shape, dtype=dtype))
+
+
+class Recorder:
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 0
+        return call
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    lib = Recorder()
+    monkeypatch.setattr(blas._lib, "lib", lambda: lib)
+    monkeypatch.setattr(blas, "_device", lambda t, name: 0)
+    monkeypatch.setattr(blas, "_stream_of", lambda dev: 0)
+    return lib.calls
+
+
+T, K, C = 6, 2, 8
+I32, F32 = torch.int32, torch.float32
+
+
+def _expert_calls(pos, weights, dweights):
+    x, xs = zeros(T, C), zeros(T * K, C)
+    yield "pos", lambda: blas.expert_sort(T, K, 4, zeros(T, K, dtype=I32), zeros(5, dtype=I32), pos)
+    yield "pos", lambda: blas.expert_gather(T, K, T * K, C, x, pos, xs)
+    yield "pos", lambda: blas.expert_combine(T, K, T * K, C, xs, pos, zeros(T, K), x)
+    yield "pos", lambda: blas.expert_combine_grad(T, K, T * K, C, x, xs, pos, None, xs, zeros(T, K))
+    good = zeros(T, K, dtype=I32)
+    yield "weights", lambda: blas.expert_combine(T, K, T * K, C, xs, good, weights, x)
+    yield "weights", lambda: blas.expert_combine_grad(T, K, T * K, C, x, xs, good, weights, xs, None)
+    yield "dweights", lambda: blas.expert_combine_grad(T, K, T * K, C, x, xs, good, None, xs, dweights)
+
+
+@pytest.mark.parametrize("shape", [(T, K), (T + 3, K), (T * K,), (T * K + 5,), (1, T, K), (T * K, 1), (1, T * K)])
+def test_a_value_per_choice(calls, shape):
+    """Rows of topk values without gaps, as the kernels read them, or the same values in one row; more of them may follow."""
+    for _, call in _expert_calls(zeros(*shape, dtype=I32), zeros(*shape), zeros(*shape)):
+        call()
+    assert len(calls) == 7
+
+
+@pytest.mark.parametrize("shape", [(T, K + 1), (K, T), (T, 2 * K), (T + 1, 1, K + 2), (T - 1, K), (T * K - 1,)])
+def test_rows_of_another_length_are_refused(calls, shape):
+    for name, call in _expert_calls(zeros(*shape, dtype=I32), zeros(*shape), zeros(*shape)):
+        with pytest.raises(blas.HpcdnnError, match=f"^{name} "):
+            call()
+    assert not calls
+
+
+def _norm_calls(mean, rstd):
+    x, y, good = zeros(T, C), zeros(T, C), zeros(T)
+    yield "mean", lambda: blas.layer_norm(T, C, x, None, None, 1e-5, y, mean, good)
+    yield "rstd", lambda: blas.layer_norm(T, C, x, None, None, 1e-5, y, good, rstd)
+    yield "mean", lambda: blas.layer_norm_grad(T, C, y, x, None, mean, good, zeros(T, C), None, None)
+    yield "rstd", lambda: blas.layer_norm_grad(T, C, y, x, None, good, rstd, zeros(T, C), None, None)
+
+
+@pytest.mark.parametrize("shape", [(T,), (T + 4,), (2, T // 2), (T, 1), (1, T + 1)])
+def test_a_value_per_row(calls, shape):
+    for _, call in _norm_calls(zeros(*shape), zeros(*shape)):
+        call()
+    assert len(calls) == 4
+
+
+@pytest.mark.parametrize("shape", [(T, 2), (2, T), (T + 2, 3), (T - 1,), (2, 2)])
+def test_more_than_a_value_per_row_is_refused(calls, shape):
+    for name, call in _norm_calls(zeros(*shape), zeros(*shape)):
+        with pytest.raises(blas.HpcdnnError, match=f"^{name} "):
+            call()
+    assert not calls
