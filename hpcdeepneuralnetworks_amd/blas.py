@@ -502,7 +502,8 @@ def w4_gemv(batch: int, M: int, N: int, group: int, alpha: float, q: torch.Tenso
             x: torch.Tensor, beta: float, y: torch.Tensor) -> None:
     """``y = alpha * x @ W.T + beta * y`` for a few rows of ``x`` (``batch`` x N) and an M x N matrix of 4-bit weights
     ``W = (q - zeros) * scales``: ``q`` is uint8 with two columns a byte (the even one in the low half) and a row stride
-    that is a multiple of 4; ``scales`` (of x's type) and ``zeros`` (uint8; None: 8) are M x ceil(N / group) with one row
+    that is a multiple of 4 (the kernels read whole dwords: of the last row too, the bytes up to a multiple of 4 have to be
+    there, whatever they hold); ``scales`` (of x's type) and ``zeros`` (uint8; None: 8) are M x ceil(N / group) with one row
     stride.  ``sgemv`` is the same product with FP32 weights."""
     t = _type(x, "x")
     dev = _device(x, "x")
@@ -518,6 +519,11 @@ def w4_gemv(batch: int, M: int, N: int, group: int, alpha: float, q: torch.Tenso
     py, ldy = _rows(y, batch, M, "y", x.dtype, dev)
     if M == 1:  # the stride of a single row says nothing
         ldq = -(-ldq // 4) * 4
+    row = -(-((N + 1) // 2) // 4) * 4
+    if q.shape[1] < row and M > 0 and N > 0:
+        held = q.untyped_storage()
+        if q.data_ptr() - held.data_ptr() + (M - 1) * ldq + row > held.nbytes():
+            raise HpcdnnError(f"q must hold {row} bytes of its last row, a multiple of 4")
     check(_lib.lib().hpcdnn_w4_gemv(t, batch, M, N, group, alpha, pq, ldq, ps, pz, ldg, px, ldx, beta, py, ldy, _stream_of(dev)), "hpcdnn_w4_gemv")
 
 

@@ -488,7 +488,8 @@ int hpcdnn_layer_norm_grad(int type, int wtype, int rows, int cols, const void* 
 /* hpcdnn_sgemv (trans = 0) for a matrix of 4-bit weights and one or a few vectors:
  *   y[t][m] = alpha * sum_n W[m][n] * x[t][n] + beta * y[t][m],   W[m][n] = (q[m][n] - z[m][n / group]) * s[m][n / group],
  * W is M x N, x is batch x N, y is batch x M.  Row m of `q` holds N values of 0 .. 15, two a byte, the even
- * column in the low half; `ldq` is its length in bytes, a multiple of 4, and q is 4-byte aligned.  `scales`
+ * column in the low half; `ldq` is its length in bytes, a multiple of 4, and q is 4-byte aligned.  Whole dwords are read:
+ * of the last row too, the bytes up to a multiple of 4 have to be there.  `scales`
  * (of `type`) and `zeros` (bytes, 0 .. 15; NULL: 8 everywhere) hold ceil(N / group) values per row with row
  * length `ldg`; group is 32, 64 or 128.  beta == 0 never reads y.  What stands behind column N in the last
  * byte and group is not used.  batch <= HPCDNN_W4_MAX_BATCH, M <= HPCDNN_W4_MAX_ROWS, N <= HPCDNN_W4_MAX_COLS.  The weights enter

@@ -94,3 +94,33 @@ def test_more_than_a_value_per_row_is_refused(calls, shape):
         with pytest.raises(blas.HpcdnnError, match=f"^{name} "):
             call()
     assert not calls
+
+
+def _w4(M, N, q, batch=1):
+    groups = -(-N // 32)
+    return lambda: blas.w4_gemv(batch, M, N, 32, 1.0, q, zeros(M, groups), None, zeros(batch, N), 0.0, zeros(batch, M))
+
+
+def bytes_(n):
+    return torch.zeros(n, dtype=torch.uint8)
+
+
+@pytest.mark.parametrize("batch", [1, 5])
+def test_a_last_row_that_ends_before_its_last_dword_is_refused(calls, batch):
+    """Its last dword is read whole: it has to lie in the memory that the tensor stands for."""
+    for M, N, q in ((1, 1002, bytes_(501).view(1, 501)), (1, 3, bytes_(2).view(1, 2)), (1, 2, bytes_(1).view(1, 1)),
+                    (3, 10, bytes_(2 * 8 + 5).as_strided((3, 5), (8, 1))), (2, 9, bytes_(4 + 8 + 7).as_strided((2, 5), (8, 1), 4)),
+                    (1, 9, bytes_(40).view(5, 8)[4:, :5].clone())):
+        with pytest.raises(blas.HpcdnnError, match="last row"):
+            _w4(M, N, gpu(q), batch)()
+    assert not calls
+
+
+@pytest.mark.parametrize("batch", [1, 5])
+def test_a_last_row_inside_its_storage(calls, batch):
+    """Narrow views of rows that go on, and rows of whole dwords."""
+    cases = ((1, 1002, bytes_(504).view(1, 504)), (1, 1002, bytes_(504).view(1, 504)[:, :501]), (3, 10, bytes_(24).view(3, 8)[:, :5]),
+             (1, 9, bytes_(40).view(5, 8)[4:, :5]), (2, 16, bytes_(16).view(2, 8)), (1, 0, bytes_(0).view(1, 0)), (0, 9, bytes_(0).view(0, 5)))
+    for M, N, q in cases:
+        _w4(M, N, gpu(q), batch)()
+    assert len(calls) == len(cases)
