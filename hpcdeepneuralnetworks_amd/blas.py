@@ -445,7 +445,7 @@ def _per_row(t: torch.Tensor | None, rows: int, name: str, dev: int):
 def _scratch(ws: torch.Tensor | None, dev: int):
     if ws is None:
         return None, 0
-    if not ws.is_contiguous() or ws.get_device() != dev:
+    if not isinstance(ws, torch.Tensor) or not ws.is_contiguous() or ws.get_device() != dev:
         raise HpcdnnError("ws must be a contiguous tensor on the current device")
     return ws.data_ptr(), ws.numel() * ws.element_size()
 
@@ -455,6 +455,8 @@ def _param_type(params, dtype: torch.dtype) -> torch.dtype:
     kind = None
     for p in params:
         if p is not None:
+            if not isinstance(p, torch.Tensor):
+                raise HpcdnnError("w, b and their gradients must be tensors or None")
             if kind is None:
                 kind = p.dtype
             if p.dtype is not kind or (kind is not torch.float32 and kind is not dtype):

@@ -124,3 +124,24 @@ def test_a_last_row_inside_its_storage(calls, batch):
     for M, N, q in cases:
         _w4(M, N, gpu(q), batch)()
     assert len(calls) == len(cases)
+
+
+@pytest.mark.parametrize("wrong", [1.0, [1.0] * C, "w", object()])
+def test_what_is_no_tensor_is_refused_as_everything_else(calls, wrong):
+    x, y, v = zeros(T, C), zeros(T, C), zeros(T)
+    ids, offsets, pos = zeros(T, K, dtype=I32), zeros(5, dtype=I32), zeros(T, K, dtype=I32)
+    q, s = gpu(torch.zeros(4, 4, dtype=torch.uint8)), zeros(4, 1)
+    for call in (lambda: blas.layer_norm(T, C, wrong, None, None, 1e-5, y), lambda: blas.layer_norm(T, C, x, None, None, 1e-5, wrong),
+                 lambda: blas.layer_norm(T, C, x, wrong, None, 1e-5, y), lambda: blas.layer_norm(T, C, x, None, wrong, 1e-5, y),
+                 lambda: blas.layer_norm(T, C, x, None, None, 1e-5, y, wrong, v),
+                 lambda: blas.layer_norm_grad(T, C, y, x, None, v, v, None, wrong, None, zeros(99)),
+                 lambda: blas.layer_norm_grad(T, C, y, x, None, v, v, None, zeros(C), None, wrong),
+                 lambda: blas.w4_gemv(1, 4, 8, 32, 1.0, wrong, s, None, x, 0.0, y), lambda: blas.w4_gemv(1, 4, 8, 32, 1.0, q, wrong, None, x, 0.0, y),
+                 lambda: blas.w4_gemv(1, 4, 8, 32, 1.0, q, s, wrong, x, 0.0, y), lambda: blas.w4_gemv(1, 4, 8, 32, 1.0, q, s, None, x, 0.0, wrong),
+                 lambda: blas.expert_sort(T, K, 4, wrong, offsets, pos), lambda: blas.expert_sort(T, K, 4, ids, offsets, pos, None, wrong),
+                 lambda: blas.expert_sort(T, K, 4, ids, wrong, pos), lambda: blas.expert_gather(T, K, T * K, C, x, wrong, x),
+                 lambda: blas.expert_combine(T, K, T, C, x, pos, wrong, y), lambda: blas.expert_combine_grad(T, K, T, C, y, x, pos, None, wrong, None),
+                 lambda: blas.w4_quantize(4, 8, 32, wrong, q, s), lambda: blas.w4_quantize(4, 8, 32, x, q, wrong)):
+        with pytest.raises(blas.HpcdnnError):
+            call()
+    assert not calls
