@@ -691,9 +691,11 @@ extern "C" int hpcdnn_w4_gemv(int type, int batch, int M, int N, int group, floa
 extern "C" int hpcdnn_w4_quantize(int type, int M, int N, int group, const float* W, int64_t ldw, uint8_t* q, int64_t ldq, void* scales,
                                   uint8_t* zeros, int64_t ldg) {
     using namespace hpcdnn;
-    if (!type_valid(type) || M < 0 || N < 0 || shift_of(group) < 0) return HPCDNN_ERR_INVALID_VALUE;
+    if (!type_valid(type) || M < 0 || N < 0 || shift_of(group) < 0 || N > HPCDNN_W4_MAX_COLS || M > HPCDNN_W4_MAX_ROWS)
+        return HPCDNN_ERR_INVALID_VALUE;
     if (M == 0 || N == 0) return HPCDNN_OK;
-    if (W == nullptr || ldw < N || q == nullptr || ldq < (N + 1) / 2 || scales == nullptr || ldg < ceil_div(N, group))
+    if (W == nullptr || !aligned(W, sizeof(float)) || ldw < N || q == nullptr || ldq < (N + 1) / 2 || scales == nullptr ||
+        !aligned(scales, type_bytes(type)) || ldg < ceil_div(N, group))
         return HPCDNN_ERR_INVALID_VALUE;
     return with_type(type, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;

@@ -502,7 +502,7 @@ int hpcdnn_w4_gemv(int type, int batch, int M, int N, int group, float alpha, co
                    const uint8_t* zeros, int64_t ldg, const void* x, int64_t ldx, float beta, void* y, int64_t ldy, void* stream);
 /* Makes such a matrix from FP32 weights, all on HOST pointers.  Symmetric (zeros == NULL): s = max |w| / 7 of the
  * group, q = 8 + w / s; with zero points: s = (max - min) / 15 of a range that includes 0, z = -min / s, q = z +
- * w / s; rounded to nearest, ties to even, and kept within 0 .. 15, with s already rounded to `type`.  Weights
+ * w / s; rounded to nearest, ties to even, and kept within 0 .. 15, with s already rounded to `type`.  M, N as above.  Weights
  * or scales that are not finite in `type` return HPCDNN_ERR_INVALID_VALUE. */
 int hpcdnn_w4_quantize(int type, int M, int N, int group, const float* W, int64_t ldw, uint8_t* q, int64_t ldq, void* scales,
                        uint8_t* zeros, int64_t ldg);
