@@ -163,7 +163,7 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(
     int64_t r = block_row + team;
     row_values<T, NV, kKind> cx((wave - first_wave) * kWave + lane, row_waves * kWave, cols), cd(cx.t, cx.n, cols);
     const float inv_cols = 1.f / static_cast<float>(cols);
-    constexpr bool kKeep = NV * kVec<T> <= 8;  // w in registers; wider rows read it again (from L2), or they would spill
+    constexpr bool kKeep = NV * kVec<T> <= 8;  // w in registers; wider rows read it again (from L2), or they would spill (FP32 beyond 8192 columns does, 7 registers)
     float wf[NV][kVec<T>], dw[NV][kVec<T>], db[NV][kVec<T>];
     if (kKeep) load_params<T, W, NV, kKind>(w, 1.f, cx, cols, wf);
 #pragma unroll

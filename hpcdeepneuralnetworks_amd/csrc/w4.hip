@@ -11,6 +11,8 @@
 //    within a factor of about five of the result.  FP32 tokens use byte-to-float conversions and q itself, on the matrix
 //    cores q - z, which BF16 holds, and three BF16 in the place of each FP32 value.
 //  - x lies in LDS in the order in which the lanes need it, its sums over 32 columns beside it.
+// Dot and matrix instructions take 16-bit values below the smallest normal number as they are, so these count in full and
+// cancel against the sums, which are formed from conversions in one form and by the matrix cores in the other.
 // Measured, one token: 16384 x 16384 FP16 in groups of 64 with zero points 28 us (5.2 TB/s), 4096 x 4096 BF16 5.3 us.
 #include <algorithm>
 #include <cmath>
@@ -223,7 +225,9 @@ __global__ __launch_bounds__(kW4MaxWaves * kWave) void w4_gemv_kernel(int batch,
 // For more tokens the products go to the matrix cores: a 16 x 16 tile of y (16 tokens by 16 rows of W) takes 32 columns per
 // instruction, and the nibbles cost the same few instructions for one token or sixteen.  A workgroup has kRowTiles tiles of
 // rows by kTokTiles of tokens; its waves split the columns between them, in runs of units of 128, and their sums meet in
-// LDS at the end (in wave order): so a narrow matrix still keeps every CU loading.
+// LDS at the end (in wave order).  Columns are not split over workgroups: a matrix of fewer than 16 rows per CU leaves CUs
+// without work (sixteen BF16 tokens by 1024 x 8192 7.6 us, on 64 of them), and every 16 or 32 tokens unpack the weights again
+// (2048 BF16 tokens by 16384 x 16384 2.8 ms, 390 TFLOP/s, a third of a plain product's rate).
 //
 // What limits it is the number of cache lines and 64-byte pieces that the loads touch: neighbouring lanes therefore load
 // neighbouring 16 bytes (four lanes a row's unit of weights, four lanes 64 bytes of a token), and the order that the
@@ -599,7 +603,9 @@ int launch_w4(int batch, int M, int N, int group_shift, float alpha, const unsig
         // Row tiles of a workgroup: it reads all of x once, which costs about as much as one of them, and the CU with the
         // most workgroups decides.  (Thirteen tokens, one / two / three / four tiles: 4096 x 8192 9.8 / 12.3 / - / 17.8 us,
         // 8192 x 8192 16.5 / 13.7 / 16.9 / 19.2 us; six by 9879 x 9920 25.0 / 30.5 / 23.9 / 28.4 us; sixteen by
-        // 16384 x 16384 64 / 44 / 53 / 39 us.)
+        // 16384 x 16384 64 / 44 / 53 / 39 us.)  The rule does not see that four tiles pass the registers in some forms of the
+        // small groups: FP16 in groups of 32 without zero points spills 45 (sixteen by 16384 x 16384 71 us, BF16 39), FP32
+        // with zero points 17 in groups of 32 and 3 in groups of 64 (70 and 61 us, in groups of 128 57).
         auto cost = [&](int row_tiles, int tok_tiles) {
             return ceil_div(ceil_div(M, 16 * row_tiles) * ceil_div(batch, 16 * tok_tiles), cus) * (row_tiles + 1);
         };

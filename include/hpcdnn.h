@@ -494,7 +494,8 @@ int hpcdnn_layer_norm_grad(int type, int wtype, int rows, int cols, const void* 
  * length `ldg`; group is 32, 64 or 128.  beta == 0 never reads y.  What stands behind column N in the last
  * byte and group is not used.  batch <= HPCDNN_W4_MAX_BATCH, M <= HPCDNN_W4_MAX_ROWS, N <= HPCDNN_W4_MAX_COLS.  The weights enter
  * exactly, but x must stay a factor of 64 below the largest FP32 number, and an infinity in x gives infinities or NaN.
- * FP32 tokens of magnitude below 2^-110 may count as the next multiple of 2^-133 towards zero. */
+ * FP32 tokens of magnitude below 2^-110 may count as the next multiple of 2^-133 towards zero; 16-bit tokens count in full down to
+ * the smallest subnormal number.  A scale that is not finite gives infinities or NaN in its row. */
 #define HPCDNN_W4_MAX_BATCH 65536
 #define HPCDNN_W4_MAX_ROWS (1 << 30)
 #define HPCDNN_W4_MAX_COLS (1 << 24)
